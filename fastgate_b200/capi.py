@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libfastgate_b200.so")
 
 FG_OK, FG_ERR_SHAPE, FG_ERR_ALIGN, FG_ERR_NULL, FG_ERR_WORKSPACE = 0, 1, 2, 3, 4
-FG_ERR_CUDA, FG_ERR_TIMEOUT, FG_ERR_PLAN, FG_ERR_NO_DEVICE = 5, 6, 7, 8
+FG_ERR_CUDA, FG_ERR_TIMEOUT, FG_ERR_PLAN, FG_ERR_NO_DEVICE, FG_ERR_INDEX = 5, 6, 7, 8, 9
 FG_OP_F16_KN, FG_OP_F16_NK, FG_OP_W8A16_NK, FG_OP_W4A16_NK = 0, 1, 2, 3
 
 # every symbol include/fastgate_b200.h declares
@@ -24,6 +24,8 @@ EXPORTS = (
     "fg_group_tiles", "fg_group_destroy", "fg_chain_table_bytes", "fg_chain_create", "fg_chain_workspace_bytes",
     "fg_chain_run", "fg_chain_grid", "fg_chain_trace_offset", "fg_chain_destroy", "fg_quantize_rows_w8", "fg_gemm_fused", "fg_linear_host",
     "fg_prepack_kn_to_nk", "fg_prepack_gate_up",
+    "fg_add_rmsnorm", "fg_kv_append_int4", "fg_kv_read_int4", "fg_kv_attention_workspace_bytes", "fg_kv_attention_workspace_init",
+    "fg_kv_attention_int4",
     "fg_trace_enable", "fg_trace_read", "fg_status_str", "fg_last_cuda_error", "fg_launch_count", "fg_version",
 )
 
@@ -127,6 +129,14 @@ def _load() -> ctypes.CDLL:
     L.fg_prepack_kn_to_nk.argtypes = [vp, vp, i, i, vp]
     L.fg_prepack_gate_up.argtypes = [vp, vp, vp, i, i, vp]
     L.fg_linear_host.argtypes = [i, vp, vp, vp, vp, vp, vp, i, i, i, vp, sz, vp]
+    ll = ctypes.c_longlong
+    L.fg_add_rmsnorm.argtypes = [vp, ll, vp, vp, vp, i, vp, i, vp, i, i, ctypes.c_float, vp]
+    L.fg_kv_append_int4.argtypes = [vp, ll, vp, ll, ll, i, i, vp, ll, i, vp, i, vp, ll, vp, i, vp, ll, vp, ll, i, i, vp, vp]
+    L.fg_kv_read_int4.argtypes = [vp, ll, i, i, i, vp, i, ll, vp, vp, vp, vp]
+    L.fg_kv_attention_workspace_bytes.argtypes = []
+    L.fg_kv_attention_workspace_bytes.restype = sz
+    L.fg_kv_attention_workspace_init.argtypes = [vp, sz, vp]
+    L.fg_kv_attention_int4.argtypes = [vp, ll, vp, ll, ll, i, i, i, vp, ll, i, vp, ll, i, vp, vp, i, ctypes.c_float, vp, vp, sz, vp]
     L.fg_trace_enable.argtypes = [i]
     L.fg_trace_read.argtypes = [vp, ctypes.POINTER(ctypes.c_ulonglong), i, vp]
     L.fg_status_str.argtypes = [i]

@@ -19,6 +19,7 @@
 #include "fg_umma_chain.cuh"
 #include "fg_umma_q.cuh"
 #include "fg_quant.cuh"
+#include "fg_host.h"
 #include "fg_layout.h"
 
 static_assert(FG_TILE_N == fg::kTileN, "layout mismatch");
@@ -490,7 +491,68 @@ int noalloc_scratch(int dev_index, unsigned char** out) {
   return FG_OK;
 }
 
+// shared memory that fg_host.h's kernels have opted in to, per device; under g_dev_mu
+struct SmemOptIn {
+  int device;
+  const void* kernel;
+  int bytes;
+};
+constexpr int kMaxSmemOptIns = 512;
+SmemOptIn g_smem_opted[kMaxSmemOptIns];
+int g_smem_opted_count = 0;
+
 }  // namespace
+
+// ---- helpers for the other translation units (fg_host.h) -----------------------------------
+namespace fg {
+namespace host {
+
+int current_device(Device* out) {
+  DeviceInfo* d = nullptr;
+  const int st = device_info(&d);
+  if (st != FG_OK) return st;
+  out->index = static_cast<int>(d - g_dev);
+  out->sm_count = d->sm_count;
+  out->smem_optin = d->smem_optin;
+  return FG_OK;
+}
+
+int encode_tensor(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, uint64_t inner, uint64_t rows,
+                  uint32_t box_inner, uint32_t box_rows) {
+  return encode_2d(tm, dt, elem_bytes, base, inner, rows, box_inner, box_rows);
+}
+
+int opt_in_smem(const void* kernel, int bytes) {
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) {
+    std::lock_guard<std::mutex> lk(g_dev_mu);
+    SmemOptIn* known = nullptr;
+    for (int i = 0; i < g_smem_opted_count; ++i)
+      if (g_smem_opted[i].device == dev && g_smem_opted[i].kernel == kernel) known = &g_smem_opted[i];
+    if (known != nullptr && bytes <= known->bytes) return FG_OK;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) {
+      if (known != nullptr) known->bytes = bytes;
+      else if (g_smem_opted_count < kMaxSmemOptIns) g_smem_opted[g_smem_opted_count++] = {dev, kernel, bytes};
+      return FG_OK;
+    }
+  }
+  g_last_cuda = static_cast<int>(e);
+  return FG_ERR_CUDA;
+}
+
+int launched(cudaError_t e) {
+  if (e != cudaSuccess) {
+    g_last_cuda = static_cast<int>(e);
+    return FG_ERR_CUDA;
+  }
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return FG_OK;
+}
+
+}  // namespace host
+}  // namespace fg
 
 extern "C" {
 
@@ -1317,6 +1379,7 @@ const char* fg_status_str(int status) {
     case FG_ERR_TIMEOUT: return "bounded device-side wait gave up";
     case FG_ERR_PLAN: return "plan is not launchable";
     case FG_ERR_NO_DEVICE: return "no sm_100 device is current";
+    case FG_ERR_INDEX: return "an index read from device memory is out of range";
     default: return "unknown status";
   }
 }

@@ -1005,7 +1005,7 @@ __global__ void __launch_bounds__(streamk_max_threads<OP, MT>(), 1)
 // then streams its first weight tiles while this kernel still waits; it touches nothing else before
 // its own griddepcontrol.wait, which returns when this kernel has completed), and this kernel itself
 // starts early and begins to look at the counters once everything before it in the stream is done.
-__global__ void fg_push_wait_kernel(const unsigned long long* flags, int world, unsigned long long target,
+static __global__ void fg_push_wait_kernel(const unsigned long long* flags, int world, unsigned long long target,
                                     int* status) {
   griddep_launch_dependents();
   griddep_wait();
@@ -1014,7 +1014,7 @@ __global__ void fg_push_wait_kernel(const unsigned long long* flags, int world, 
 }
 // The same with the target read from device memory (the running total that pushing launches keep
 // in *target_dev): nothing in the launch changes from call to call, so it can be replayed in a graph.
-__global__ void fg_push_wait_dev_kernel(const unsigned long long* flags, int world,
+static __global__ void fg_push_wait_dev_kernel(const unsigned long long* flags, int world,
                                         const unsigned long long* target_dev, int* status) {
   griddep_launch_dependents();
   griddep_wait();  // the launches that add to *target_dev have completed
@@ -1031,7 +1031,7 @@ struct WaitList {
   const unsigned long long* target_dev[kMaxWaits];
   int count;
 };
-__global__ void fg_push_wait_many_kernel(const WaitList w, int world, int* status) {
+static __global__ void fg_push_wait_many_kernel(const WaitList w, int world, int* status) {
   griddep_launch_dependents();
   griddep_wait();
   const int i = threadIdx.x;

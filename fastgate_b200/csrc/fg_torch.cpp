@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "../../include/fastgate_b200.h"
+#include "fg_torch.h"
 
 namespace {
 
@@ -453,6 +454,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "W[N,K] fp16 -> (W4 [N,K/2] uint8, scales [N, K/group_size] fp16), zero point 8, for fastgemv_int4");
   m.def("quantize_int8", &quantize_int8, py::arg("W"),
         "W[N,K] fp16 -> (W8 int8, scales fp16): symmetric, one scale per output channel, for fastgemv_int8");
+  bind_serving(m);
   m.def("launch_count", []() { return fg_launch_count(); });
   m.def("version", []() { return std::string(fg_version()); });
 }

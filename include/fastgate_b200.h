@@ -48,7 +48,9 @@ enum {
   FG_ERR_CUDA = 5,      /* a CUDA runtime/driver call failed (see fg_last_cuda_error) */
   FG_ERR_TIMEOUT = 6,   /* a bounded device-side wait gave up (read back with fg_workspace_status) */
   FG_ERR_PLAN = 7,      /* a caller-supplied plan is not launchable            */
-  FG_ERR_NO_DEVICE = 8  /* no sm_100 device is current                         */
+  FG_ERR_NO_DEVICE = 8, /* no sm_100 device is current                         */
+  FG_ERR_INDEX = 9      /* a kernel met an index (slot, page, position, length) out of range in device memory: the
+                           access was left out and the status word set (never returned by a call) */
 };
 
 /* ---- operand layouts ------------------------------------------------------ */
@@ -365,6 +367,69 @@ int fg_prepack_gate_up(const void* Wg, const void* Wu, void* Wgu, int Nh, int K,
  * W8 = clamp(rint(W / scale), -127, 127).  K % 8 == 0.  The reference has no quantiser (its
  * int8 GEMV is fed hand-made data, script/fastgemv-int8.py:5-11). */
 int fg_quantize_rows_w8(const void* W, int8_t* W8, void* scales, int N, int K, fg_stream_t stream);
+
+/* ---- RMS norm with the residual addition ---------------------------------------------------
+ * For every row m of x[M,K] (fp16, row stride ldx elements), with h = x[m] (+ residual[m]):
+ *     residual_out[m] = h                       (rounded once to the residual's type)
+ *     rstd = 1 / sqrt(mean_k h^2 + eps)
+ *     out[m] = h * rstd * weight                (out_int8 == 0: fp16, rounded once)
+ *     out[m] = rint(t * (127 / a)), scales[m] = a * rstd / 127   with t = h * weight, a = max|t|
+ *                                               (out_int8 == 1: the activations of fg_linear_w8a8)
+ * rstd cancels out of the int8 codes, so they do not depend on the order of the sum of squares.  A row whose t is
+ * all zero gets codes 0 and scale 1 (as in fg_quantize_rows_w8); one with an infinity or a NaN gets a NaN scale.
+ * weight [K] fp16; residual and residual_out [M,K] dense, fp16 or (residual_f32 == 1) fp32, both NULL or neither; they
+ * may be the same buffer.  An fp16 out may be x itself.  K % 8 == 0, M >= 1.  Sums in fp32.  No counterpart in the
+ * reference (it has no norm). */
+int fg_add_rmsnorm(const void* x, long long ldx, const void* weight, const void* residual, void* residual_out,
+                   int residual_f32, void* out, int out_int8, float* scales, int M, int K, float eps, fg_stream_t stream);
+
+/* ---- key/value cache held in 4 bits -------------------------------------------------------
+ * What a decode step needs between the fused QKV projection and the output projection.  The cache is a pool of
+ * `num_pages` pages; a page holds page_size rows (a multiple of 16) for each of kv_heads heads of d = 64 or 128
+ * channels, kv_heads * page_size * (d + 8) bytes.  Within a head's part of a page the rows lie in blocks of 16:
+ *     [16][d/2] key codes | [16][d/2] value codes | [16] key parameters | [16] value parameters
+ * codes two per byte, low nibble = even channel (as in fg_quantize_rows_w4); parameters a (scale, low) pair of fp16; the
+ * row that is stored is low + scale * code.  Row r of page i is "slot" i * page_size + r.  pages: 16-byte aligned.
+ *
+ * Indices that lie in device memory (slots, positions, page numbers, lengths) are checked by the kernels: an access out
+ * of range is left out and FG_ERR_INDEX stored to *status_dev (int in device memory, or NULL: not reported).
+ *
+ * fg_kv_append_int4: for each of `tokens` rows t with slots[t] >= 0 (negative: a padding row, left out whole), turns
+ * k[t] and q[t] by the angles of positions[t], writes q to q_out (fp16, rounded once; q_out may be q) and the rows
+ * k[t], v[t] of every head, quantised from the unrounded values, to the cache:
+ *     low = fp16(min x), scale = max(fp16((max x - low) / 15), 2^-24), code = clamp(rint((x - low) / scale), 0, 15)
+ * A row with an infinity or a NaN in it reads back as NaN.  k, v [tokens, kv_heads, d] and q, q_out
+ * [tokens, q_heads, d] fp16 with token strides ldk, ldv, ldq, ldqo (elements, multiples of 8), heads dense: column ranges
+ * of one fused projection serve as they are.  cos_sin [positions_len, d] fp32 holds cos of the d/2 angles of a position,
+ * then sin; interleaved = 0 turns channel pairs (i, i + d/2), 1 pairs (2i, 2i + 1).  cos_sin and positions NULL: no
+ * rotation (and no q).  slots and positions are int32 or (slots_64, positions_64) int64.  The slots >= 0 of one call
+ * must differ from one another: of two rows in one slot, what is left there is unspecified. */
+int fg_kv_append_int4(const void* k, long long ldk, const void* v, long long ldv, long long tokens, int kv_heads, int d,
+                      void* pages, long long num_pages, int page_size, const void* slots, int slots_64, const float* cos_sin,
+                      long long positions_len, const void* positions, int positions_64, const void* q, long long ldq,
+                      void* q_out, long long ldqo, int q_heads, int interleaved, int* status_dev, fg_stream_t stream);
+
+/* The rows of `slots` as fp16: k_out, v_out [tokens, kv_heads, d] dense.  Rows of a negative slot are left as they were. */
+int fg_kv_read_int4(const void* pages, long long num_pages, int page_size, int kv_heads, int d, const void* slots,
+                    int slots_64, long long tokens, void* k_out, void* v_out, int* status_dev, fg_stream_t stream);
+
+/* Attention of new tokens over the cache.  q, out [tokens, q_heads, d] fp16 (token strides ldq, ldo in elements); query
+ * head h reads key/value head h / (q_heads / kv_heads).  Sequence b has seq_lens[b] rows in the cache, its new tokens
+ * among them, in the pages block_table[b * ldt + 0 ..] (table_width of them at most), and the query rows
+ * q_starts[b] .. q_starts[b+1] - 1 (q_starts NULL: tokens == batch, row b).  Its i-th of n query rows is at position
+ * seq_lens[b] - n + i and sees the rows up to there:
+ *     out = sum_t softmax_t(scale * q . k_t) v_t
+ * A query that sees nothing (an empty sequence) gives zeros; rows of q outside every sequence leave out as it was; rows of
+ * a page number out of range count as absent.  Scores, weights and sums in fp32, weights rounded to fp16 for the product
+ * with the codes.  The split over the length depends on the lengths alone: results are reproducible bit by bit.
+ * ws: fg_kv_attention_workspace_bytes() of device memory, 256-byte aligned, cleared once with
+ * fg_kv_attention_workspace_init (a call leaves it ready for the next); one per stream that may run concurrently. */
+size_t fg_kv_attention_workspace_bytes(void);
+int fg_kv_attention_workspace_init(void* ws, size_t ws_bytes, fg_stream_t stream);
+int fg_kv_attention_int4(const void* q, long long ldq, void* out, long long ldo, long long tokens, int q_heads, int kv_heads, int d,
+                         const void* pages, long long num_pages, int page_size, const int* block_table, long long ldt,
+                         int table_width, const int* seq_lens, const int* q_starts, int batch, float scale, int* status_dev,
+                         void* ws, size_t ws_bytes, fg_stream_t stream);
 
 /* ---- end-to-end convenience (HOST pointers) ---------------------------------
  * x_host and C_host are host buffers (pinned for full speed); W_dev, scales_dev,
