@@ -1,5 +1,5 @@
 // pybind11 / torch-extension surface of the operators that stand around the linears in a serving step: RMS norm,
-// 4-bit key/value cache.  Thin layers over the C ABI, like fg_torch.cpp: tensor checks, the current
+// linear on 8-bit activations, 4-bit key/value cache.  Thin layers over the C ABI, like fg_torch.cpp: tensor checks, the current
 // stream of the tensors' device, workspaces, status codes as exceptions.  There is no CPU path.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -130,6 +130,63 @@ void add_rmsnorm(at::Tensor x, at::Tensor weight, at::Tensor out, OptTensor resi
   check_status(st);
 }
 
+// ---- linear on 8-bit activations -------------------------------------------------------------
+bool capturing(cudaStream_t stream) {
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(stream, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone;
+}
+
+void linear_int8(at::Tensor x8, at::Tensor W8, at::Tensor C, at::Tensor x_scales, OptTensor w_scales, OptTensor bias, OptTensor residual,
+                 const std::string& act) {
+  int code;
+  if (act == "none") code = FG_ACT_NONE;
+  else if (act == "gelu" || act == "gelu_erf") code = FG_ACT_GELU_ERF;
+  else if (act == "gelu_tanh") code = FG_ACT_GELU_TANH;
+  else if (act == "silu") code = FG_ACT_SILU;
+  else if (act == "silu_gate") code = FG_ACT_SILU_GATE;
+  else throw std::invalid_argument("fastgate_b200: act must be none, gelu, gelu_tanh, silu or silu_gate");
+  check_dense(x8, "activation", at::kChar, -1);
+  const int64_t device = x8.get_device();
+  check_dense(W8, "weight", at::kChar, device);
+  check_dense(C, "output", at::kHalf, device);
+  if (x8.dim() != 2 || W8.dim() != 2) throw std::runtime_error("fastgate_b200: activation and weight must be 2-D");
+  const int64_t M = x8.size(0), K = x8.size(1), N = W8.size(0);
+  if (W8.size(1) != K) throw std::runtime_error("fastgate_b200: activation and weight disagree on K");
+  const int64_t width = code == FG_ACT_SILU_GATE ? N / 2 : N;
+  if (C.numel() != M * width) throw std::runtime_error("fastgate_b200: output must hold M*N elements (M*N/2 with silu_gate)");
+  const bool f32 = x_scales.defined() && x_scales.scalar_type() == at::kFloat;
+  check_dense(x_scales, "x_scales", f32 ? at::kFloat : at::kHalf, device);
+  if (x_scales.numel() != M) throw std::runtime_error("fastgate_b200: x_scales must hold M elements");
+  auto optional_half = [&](const OptTensor& t, const char* name, int64_t n) -> const void* {
+    if (!given(t)) return nullptr;
+    check_dense(*t, name, at::kHalf, device);
+    if (t->numel() != n) throw std::runtime_error(std::string("fastgate_b200: ") + name + " must hold " + std::to_string(n) + " elements");
+    return t->data_ptr();
+  };
+  const void* ws_ptr = optional_half(w_scales, "w_scales", N);
+  const void* bias_ptr = optional_half(bias, "bias", N);
+  const void* res_ptr = optional_half(residual, "residual", M * width);
+  if (M == 0) return;
+  if ((N % 128) != 0 || (K % 128) != 0 || N <= 0 || K <= 0)
+    throw std::invalid_argument("K(input column) & N(transposed output row) must be multiple of 128!");
+  if (K > 131072 - 128) bad_argument("K must be at most 130944: the sums are 32-bit integers");
+  if (M > 0x7fffffff || N > 0x7fffffff) bad_argument("too many rows");
+  if (overlap(C, x8) || overlap(C, W8) || overlap(C, x_scales) || (given(w_scales) && overlap(C, *w_scales)) || (given(bias) && overlap(C, *bias)) ||
+      (given(residual) && overlap(C, *residual) && C.data_ptr() != residual->data_ptr()))
+    bad_argument("the output may be the residual itself; otherwise it must not overlap the inputs");
+  const c10::cuda::CUDAGuard guard(x8.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
+  const StreamWorkspace ws = capturing(stream) ? captured_workspace(device, stream, N) : stream_workspace(device, stream, N);
+  int st;
+  {
+    pybind11::gil_scoped_release nogil;
+    st = fg_linear_w8a8(static_cast<const int8_t*>(x8.data_ptr()), static_cast<const int8_t*>(W8.data_ptr()), x_scales.data_ptr(), f32, ws_ptr,
+                        C.data_ptr(), static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), bias_ptr, res_ptr, code,
+                        ws.buf.data_ptr(), ws.bytes, reinterpret_cast<fg_stream_t>(stream));
+  }
+  check_status(st);
+}
+
 // ---- 4-bit key/value cache -----------------------------------------------------------------
 // pages [num_pages, kv_heads, page_size * (D + 8)] uint8
 void check_pages(const at::Tensor& pages, int64_t page_size, int64_t kv_heads, int64_t d, int64_t device) {
@@ -222,11 +279,6 @@ void kv_read_int4(at::Tensor pages, at::Tensor slots, at::Tensor k_out, at::Tens
 std::mutex g_attn_mu;
 std::map<std::pair<int64_t, int64_t>, at::Tensor> g_attn_ws;
 
-bool capturing(cudaStream_t stream) {
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  return cudaStreamIsCapturing(stream, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone;
-}
-
 // One workspace per (device, stream), made on the first call.  A call that is being captured gets one of its own from the
 // graph's memory, cleared inside the graph: two graphs captured on one stream may be replayed side by side.
 at::Tensor attention_workspace(int64_t device, cudaStream_t stream) {
@@ -302,6 +354,10 @@ void bind_serving(pybind11::module& m) {
         py::arg("eps") = 1e-6, py::arg("scales") = py::none(), py::arg("residual_out") = py::none(),
         "h = x (+ residual); residual_out (default: residual, in place) = h; out = h / sqrt(mean h^2 + eps) * weight.  x [M,K] fp16; "
         "residual fp16 or fp32; out fp16, or int8 with one fp32 scale per row in `scales` (the activations of linear_int8)");
+  m.def("linear_int8", &linear_int8, py::arg("x8"), py::arg("W8"), py::arg("C"), py::arg("x_scales"), py::arg("w_scales") = py::none(),
+        py::arg("bias") = py::none(), py::arg("residual") = py::none(), py::arg("act") = "none",
+        "C[M,N] = act(x8 . W8^T * x_scales[m] * w_scales[n] + bias) + residual: int8 x8 [M,K] (add_rmsnorm, quantize_int8) and W8 [N,K], exact "
+        "integer sums; x_scales fp32 or fp16, the rest fp16; act='silu_gate': C[M,N/2] on a weight from prepack_gate_up");
   m.def("kv_append_int4", &kv_append_int4, py::arg("k"), py::arg("v"), py::arg("pages"), py::arg("slots"), py::arg("page_size"),
         py::arg("cos_sin") = py::none(), py::arg("positions") = py::none(), py::arg("q") = py::none(), py::arg("q_out") = py::none(),
         py::arg("interleaved") = false, py::arg("status") = py::none(),

@@ -15,8 +15,8 @@ multiple of 128 (hk/edgemm.cu:107-109).  Ops that took a split-K hint ``bz`` sti
 [N, K/128]); the reference has the kernel (hk/fastgemv.cuh:394-495) but no operator for it.
 
 ``SERVING`` names the operators that stand around the linears in a serving step (no counterpart in the
-reference): ``add_rmsnorm`` (residual addition, RMS norm, fp16 or int8 rows with scales) and the paged
-key/value cache in 4 bits, ``kv_append_int4``, ``kv_read_int4`` and ``kv_attention_int4``
+reference): ``add_rmsnorm`` (residual addition, RMS norm, fp16 or int8 rows with scales), ``linear_int8`` (int8
+activations and weights, bias, activation, residual) and the paged key/value cache in 4 bits, ``kv_append_int4``, ``kv_read_int4`` and ``kv_attention_int4``
 (``fastgate_b200.kvcache.KVCacheInt4`` keeps the pool and its bookkeeping).
 """
 from . import _C
@@ -41,7 +41,7 @@ COMPARATORS = ("hgemm", "hgemm_tr")
 EXTRA = ("linear_nk_push", "push_wait", "push_wait_dev", "push_wait_dev_many", "workspace_status", "quantize_int8", "linear_fused", "fastgemv_int4",
          "quantize_int4", "prepack_kn_to_nk", "prepack_gate_up")
 # what stands around the linears in a serving step with 8-bit activations and a 4-bit key/value cache
-SERVING = ("add_rmsnorm", "kv_append_int4", "kv_read_int4", "kv_attention_int4")
+SERVING = ("add_rmsnorm", "linear_int8", "kv_append_int4", "kv_read_int4", "kv_attention_int4")
 
 __all__ = list(KN_OPS + NK_OPS + WF_OPS + COMPARATORS + EXTRA + SERVING) + ["launch_count", "version",
                                                          "KN_OPS", "NK_OPS", "WF_OPS", "BZ_OPS"]

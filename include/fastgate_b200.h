@@ -383,6 +383,19 @@ int fg_quantize_rows_w8(const void* W, int8_t* W8, void* scales, int N, int K, f
 int fg_add_rmsnorm(const void* x, long long ldx, const void* weight, const void* residual, void* residual_out,
                    int residual_f32, void* out, int out_int8, float* scales, int M, int K, float eps, fg_stream_t stream);
 
+/* ---- linear on 8-bit activations ------------------------------------------------------------
+ * x8[M,K] int8 with one scale per row (fg_add_rmsnorm, or fg_quantize_rows_w8 on the activations) and W8[N,K] int8 with one
+ * fp16 scale per output channel (NULL: 1):
+ *     C[m,n] = act(x_scales[m] * w_scales[n] * sum_k x8[m,k] W8[n,k] + bias[n]) + residual[m,n]
+ * x_scales fp32 (x_scales_f32 == 1) or fp16; bias [N], residual and C fp16; act FG_ACT_*.  With FG_ACT_SILU_GATE W8 holds 64
+ * gate rows, then the matching 64 up rows, per 128 (fg_prepack_gate_up on the two int8 weights with K/2 for K); C and
+ * residual are [M, N/2].  The sums are exact 32-bit integers: a row's result depends neither on the rows beside it nor on how
+ * the work is split.  K, N % 128 == 0, K <= 130944 (where the sums still fit), any M >= 1.  Workspace as for the other
+ * linears.  residual may be C. */
+int fg_linear_w8a8(const int8_t* x8, const int8_t* W8, const void* x_scales, int x_scales_f32, const void* w_scales, void* C,
+                   int M, int N, int K, const void* bias, const void* residual, int act, void* ws, size_t ws_bytes,
+                   fg_stream_t stream);
+
 /* ---- key/value cache held in 4 bits -------------------------------------------------------
  * What a decode step needs between the fused QKV projection and the output projection.  The cache is a pool of
  * `num_pages` pages; a page holds page_size rows (a multiple of 16) for each of kv_heads heads of d = 64 or 128
