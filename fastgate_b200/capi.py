@@ -23,7 +23,7 @@ EXPORTS = (
     "fg_gemm_f16_nk_push", "fg_push_wait", "fg_push_wait_dev", "fg_push_wait_dev_many", "fg_group_table_bytes", "fg_group_create", "fg_group_run",
     "fg_group_tiles", "fg_group_destroy", "fg_chain_table_bytes", "fg_chain_create", "fg_chain_workspace_bytes",
     "fg_chain_run", "fg_chain_grid", "fg_chain_trace_offset", "fg_chain_destroy", "fg_quantize_rows_w8", "fg_gemm_fused", "fg_linear_host",
-    "fg_prepack_kn_to_nk", "fg_prepack_gate_up",
+    "fg_prepack_kn_to_nk", "fg_prepack_gate_up", "fg_prepack_gate_up_w8",
     "fg_add_rmsnorm", "fg_linear_w8a8", "fg_kv_append_int4", "fg_kv_read_int4", "fg_kv_attention_workspace_bytes", "fg_kv_attention_workspace_init",
     "fg_kv_attention_int4",
     "fg_trace_enable", "fg_trace_read", "fg_status_str", "fg_last_cuda_error", "fg_launch_count", "fg_version",
@@ -128,9 +128,11 @@ def _load() -> ctypes.CDLL:
     L.fg_gemm_fused.argtypes = [i, vp, vp, vp, vp, i, i, i, ctypes.POINTER(Epilogue), vp, sz, vp]
     L.fg_prepack_kn_to_nk.argtypes = [vp, vp, i, i, vp]
     L.fg_prepack_gate_up.argtypes = [vp, vp, vp, i, i, vp]
+    L.fg_prepack_gate_up_w8.argtypes = [vp, vp, vp, i, i, vp]
     L.fg_linear_host.argtypes = [i, vp, vp, vp, vp, vp, vp, i, i, i, vp, sz, vp]
     ll = ctypes.c_longlong
     L.fg_add_rmsnorm.argtypes = [vp, ll, vp, vp, vp, i, vp, i, vp, i, i, ctypes.c_float, vp]
+    L.fg_plan_w8a8.argtypes = [i, i, i, i, i, i, ctypes.POINTER(Plan)]  # internal: the streaming kernel of fg_linear_w8a8
     L.fg_linear_w8a8.argtypes = [vp, vp, vp, i, vp, vp, i, i, i, vp, vp, i, vp, sz, vp]
     L.fg_kv_append_int4.argtypes = [vp, ll, vp, ll, ll, i, i, vp, ll, i, vp, i, vp, ll, vp, i, vp, ll, vp, ll, i, i, vp, vp]
     L.fg_kv_read_int4.argtypes = [vp, ll, i, i, i, vp, i, ll, vp, vp, vp, vp]

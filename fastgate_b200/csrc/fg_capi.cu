@@ -1195,12 +1195,12 @@ int fg_prepack_kn_to_nk(const void* B, void* W, int N, int K, fg_stream_t stream
   return FG_OK;
 }
 
-int fg_prepack_gate_up(const void* Wg, const void* Wu, void* Wgu, int N, int K, fg_stream_t stream) {
+static int interleave_gate_up(const void* Wg, const void* Wu, void* Wgu, int N, int K, int elem_bytes, fg_stream_t stream) {
   if (Wg == nullptr || Wu == nullptr || Wgu == nullptr) return FG_ERR_NULL;
   if (N <= 0 || K <= 0 || (N % 64) != 0 || (K % 128) != 0) return FG_ERR_SHAPE;
   if (!aligned16(Wg) || !aligned16(Wu) || !aligned16(Wgu)) return FG_ERR_ALIGN;
   // blocks of 64 rows are contiguous in all three matrices: 2 * N / 64 plain copies as one kernel
-  const long long chunks16 = static_cast<long long>(64) * K * 2 / 16;  // 16-byte pieces per block of rows
+  const long long chunks16 = static_cast<long long>(64) * K * elem_bytes / 16;  // 16-byte pieces per block of rows
   const dim3 grid(static_cast<unsigned>((chunks16 + 1023) / 1024), 2 * (N / 64));
   fg::fg_interleave_gate_up_kernel<<<grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       static_cast<const uint4*>(Wg), static_cast<const uint4*>(Wu), static_cast<uint4*>(Wgu), static_cast<int>(chunks16));
@@ -1211,6 +1211,14 @@ int fg_prepack_gate_up(const void* Wg, const void* Wu, void* Wgu, int N, int K, 
   }
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return FG_OK;
+}
+
+int fg_prepack_gate_up(const void* Wg, const void* Wu, void* Wgu, int N, int K, fg_stream_t stream) {
+  return interleave_gate_up(Wg, Wu, Wgu, N, K, 2, stream);
+}
+
+int fg_prepack_gate_up_w8(const void* Wg, const void* Wu, void* Wgu, int N, int K, fg_stream_t stream) {
+  return interleave_gate_up(Wg, Wu, Wgu, N, K, 1, stream);
 }
 
 int fg_linear_host(int op, const void* x_host, const void* W_dev, const void* scales_dev, void* C_host,

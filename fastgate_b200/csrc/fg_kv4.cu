@@ -231,7 +231,11 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_read_kernel(const ReadParams
         const float scale = __low2float(par[i][which]), low = __high2float(par[i][which]);
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = fmaf(static_cast<float>((w[i][which] >> (4 * j)) & 15u), scale, low);
+        for (int j = 0; j < 8; ++j) {
+          // at the ends of fp16's range the rounded scale may carry the top code past 65504: it saturates (NaN stays NaN)
+          const float f = fmaf(static_cast<float>((w[i][which] >> (4 * j)) & 15u), scale, low);
+          v[j] = f > 65504.f ? 65504.f : f;
+        }
         __half* dst = (which ? p.v : p.k) + (token * p.kv.heads + head0 + i) * D + 8 * lane;
         *reinterpret_cast<uint4*>(dst) = pack8(v);
       }

@@ -341,17 +341,24 @@ at::Tensor prepack_kn_to_nk(at::Tensor B) {
   return W;
 }
 
-// Wg[N,K], Wu[N,K] fp16 -> Wgu[2N,K] fp16, blocks of 64 rows interleaved (gate first).
+// Wg[N,K], Wu[N,K] fp16 or int8 -> Wgu[2N,K], blocks of 64 rows interleaved (gate first).  Vectors of N elements (the two
+// projections' biases or channel scales) are brought into the same order.
 at::Tensor prepack_gate_up(at::Tensor Wg, at::Tensor Wu) {
-  check_tensor(Wg, "gate weight", at::kHalf);
-  check_tensor(Wu, "up weight", at::kHalf);
+  const bool int8w = Wg.scalar_type() == at::kChar;
+  check_tensor(Wg, "gate weight", int8w ? at::kChar : at::kHalf);
+  check_tensor(Wu, "up weight", int8w ? at::kChar : at::kHalf);
+  if (!int8w && Wg.dim() == 1) {
+    if (Wg.sizes() != Wu.sizes() || (Wg.size(0) % 64) != 0) throw std::invalid_argument("fastgate_b200: gate and up vectors of one length, a multiple of 64, expected");
+    return at::stack({Wg.view({-1, 64}), Wu.view({-1, 64})}, 1).reshape({-1});
+  }
   if (Wg.dim() != 2 || Wg.sizes() != Wu.sizes() || (Wg.size(0) % 64) != 0 || (Wg.size(1) % 128) != 0)
     throw std::invalid_argument("fastgate_b200: gate and up weights [N,K] of one shape, N % 64 == 0, K % 128 == 0 expected");
   const c10::cuda::CUDAGuard guard(Wg.device());
   at::Tensor Wgu = at::empty({2 * Wg.size(0), Wg.size(1)}, Wg.options());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(Wg.get_device()).stream();
-  const int st = fg_prepack_gate_up(Wg.data_ptr(), Wu.data_ptr(), Wgu.data_ptr(), static_cast<int>(Wg.size(0)),
-                                    static_cast<int>(Wg.size(1)), reinterpret_cast<fg_stream_t>(stream));
+  const auto prepack = int8w ? &fg_prepack_gate_up_w8 : &fg_prepack_gate_up;
+  const int st = prepack(Wg.data_ptr(), Wu.data_ptr(), Wgu.data_ptr(), static_cast<int>(Wg.size(0)),
+                         static_cast<int>(Wg.size(1)), reinterpret_cast<fg_stream_t>(stream));
   if (st != FG_OK) raise(st, true);
   return Wgu;
 }
@@ -457,7 +464,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("workspace_status", &workspace_status, py::arg("device"));
   m.def("prepack_kn_to_nk", &prepack_kn_to_nk, py::arg("B"), "B[K,N] fp16 -> W[N,K] fp16 (one-time repack for the NxK operators)");
   m.def("prepack_gate_up", &prepack_gate_up, py::arg("Wg"), py::arg("Wu"),
-        "Wg[N,K], Wu[N,K] fp16 -> Wgu[2N,K]: 64 gate rows, then the matching 64 up rows, per 128 rows (for act='silu_gate')");
+        "Wg[N,K], Wu[N,K] fp16 or int8 -> Wgu[2N,K]: 64 gate rows, then the matching 64 up rows, per 128 rows (for act='silu_gate'); two "
+        "fp16 vectors of N elements (biases, channel scales) into the same order");
   m.def("linear_fused", &linear_fused, py::arg("x"), py::arg("W"), py::arg("C"), py::arg("scales") = py::none(),
         py::arg("bias") = py::none(), py::arg("residual") = py::none(), py::arg("act") = "none", py::arg("layout") = "nk",
         py::arg("C2") = py::none(), py::arg("C3") = py::none(),

@@ -360,6 +360,8 @@ int fg_gemm_fused(int op, const void* x, const void* W, const void* scales, void
  * followed by the matching 64 up rows (Nh a multiple of 64): the weight FG_ACT_SILU_GATE takes. */
 int fg_prepack_kn_to_nk(const void* B, void* W, int N, int K, fg_stream_t stream);
 int fg_prepack_gate_up(const void* Wg, const void* Wu, void* Wgu, int Nh, int K, fg_stream_t stream);
+/* The same for int8 weights (fg_linear_w8a8). */
+int fg_prepack_gate_up_w8(const void* Wg, const void* Wu, void* Wgu, int Nh, int K, fg_stream_t stream);
 
 /* ---- int8 weight producer ----------------------------------------------------------------
  * Per-output-channel symmetric quantiser for fg_gemm_w8a16_nk: W[N,K] fp16 -> W8[N,K] int8
@@ -388,7 +390,7 @@ int fg_add_rmsnorm(const void* x, long long ldx, const void* weight, const void*
  * fp16 scale per output channel (NULL: 1):
  *     C[m,n] = act(x_scales[m] * w_scales[n] * sum_k x8[m,k] W8[n,k] + bias[n]) + residual[m,n]
  * x_scales fp32 (x_scales_f32 == 1) or fp16; bias [N], residual and C fp16; act FG_ACT_*.  With FG_ACT_SILU_GATE W8 holds 64
- * gate rows, then the matching 64 up rows, per 128 (fg_prepack_gate_up on the two int8 weights with K/2 for K); C and
+ * gate rows, then the matching 64 up rows, per 128 (fg_prepack_gate_up_w8; w_scales and bias in the same order); C and
  * residual are [M, N/2].  The sums are exact 32-bit integers: a row's result depends neither on the rows beside it nor on how
  * the work is split.  K, N % 128 == 0, K <= 130944 (where the sums still fit), any M >= 1.  Workspace as for the other
  * linears.  residual may be C. */
@@ -422,7 +424,8 @@ int fg_kv_append_int4(const void* k, long long ldk, const void* v, long long ldv
                       long long positions_len, const void* positions, int positions_64, const void* q, long long ldq,
                       void* q_out, long long ldqo, int q_heads, int interleaved, int* status_dev, fg_stream_t stream);
 
-/* The rows of `slots` as fp16: k_out, v_out [tokens, kv_heads, d] dense.  Rows of a negative slot are left as they were. */
+/* The rows of `slots` as fp16 (a top code that the rounded scale carries past 65504 reads as 65504): k_out, v_out
+ * [tokens, kv_heads, d] dense.  Rows of a negative slot are left as they were. */
 int fg_kv_read_int4(const void* pages, long long num_pages, int page_size, int kv_heads, int d, const void* slots,
                     int slots_64, long long tokens, void* k_out, void* v_out, int* status_dev, fg_stream_t stream);
 

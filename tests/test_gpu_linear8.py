@@ -1,0 +1,206 @@
+"""linear_int8 against 64 bits: streaming and paired kernels, every epilogue, the largest sums, splits and graphs."""
+import ctypes
+
+import pytest
+import torch
+
+import fastgate_b200 as fg
+from fastgate_b200 import capi
+from tests import serving_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda:0")
+
+
+def _data(M, N, K, seed, lim=127):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(-lim, lim + 1, (M, K), generator=g, dtype=torch.int8)
+    w = torch.randint(-lim, lim + 1, (N, K), generator=g, dtype=torch.int8)
+    sx = (torch.rand(M, generator=g) + 0.5) / 64
+    sw = ((torch.rand(N, generator=g) + 0.5) / (64 * K ** 0.5)).half()
+    return x, w, sx, sw, g
+
+
+def _check(got, want, size):
+    # the sum is exact; scales, bias, activation and residual take a few 32-bit roundings of terms of `size`
+    tol = want.abs() * ref.HALF_STEP + size * 2.0 ** -20 + ref.TINY
+    err = (got.cpu().to(torch.float64) - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("M", [1, 2, 16, 17, 33, 64, 65, 128, 129, 300])
+@pytest.mark.parametrize("N,K", [(128, 128), (1152, 640), (256, 4096), (4224, 1408)])
+def test_plain(M, N, K, dev):
+    x, w, sx, sw, _ = _data(M, N, K, M + N)
+    out = torch.full((M + 2, N), 123.0, dtype=torch.half, device=dev)
+    fg.linear_int8(x.to(dev), w.to(dev), out[1:-1], sx.to(dev), sw.to(dev))
+    _check(out[1:-1], *ref.linear_int8(x, w, sx, sw))
+    assert bool((out[0] == 123).all()) and bool((out[-1] == 123).all())
+
+
+@pytest.mark.parametrize("act", ["none", "gelu", "gelu_tanh", "silu", "silu_gate"])
+@pytest.mark.parametrize("M", [1, 40, 100, 700])
+def test_epilogues(M, act, dev):
+    N, K = 896, 512
+    x, w, sx, sw, g = _data(M, N, K, M)
+    width = N // 2 if act == "silu_gate" else N
+    bias, res = torch.randn(N, generator=g).half(), torch.randn(M, width, generator=g).half()
+    for b, r in ((bias, res), (None, res), (bias, None)):
+        out = torch.empty(M, width, dtype=torch.half, device=dev)
+        fg.linear_int8(x.to(dev), w.to(dev), out, sx.to(dev), sw.to(dev), None if b is None else b.to(dev), None if r is None else r.to(dev), act)
+        _check(out, *ref.linear_int8(x, w, sx, sw, b, r, act))
+
+
+@pytest.mark.parametrize("M", [3, 700])
+def test_scales_of_both_types_and_none(M, dev):
+    x, w, sx, sw, _ = _data(M, 384, 256, 5, lim=3)
+    h = sx.half()
+    out = torch.empty(M, 384, dtype=torch.half, device=dev)
+    fg.linear_int8(x.to(dev), w.to(dev), out, h.to(dev))
+    _check(out, *ref.linear_int8(x, w, h))
+    fg.linear_int8(x.to(dev), w.to(dev), out, h.to(dev), sw.to(dev))
+    _check(out, *ref.linear_int8(x, w, h, sw))
+
+
+@pytest.mark.parametrize("M", [1, 200, 600])
+def test_largest_sums(M, dev):
+    """All -128 at the longest K allowed: the sum is 128 * 128 * 130944, just inside 32 bits."""
+    K, N = 130944, 256
+    x = torch.full((M, K), -128, dtype=torch.int8, device=dev)
+    w = torch.full((N, K), -128, dtype=torch.int8, device=dev)
+    w[1] = 127
+    sx = torch.full((M,), 2.0 ** -20, device=dev)
+    out = torch.empty(M, N, dtype=torch.half, device=dev)
+    fg.linear_int8(x, w, out, sx)
+    want = torch.full((M, N), 128.0 * 128 * K / 2 ** 20, dtype=torch.float64)
+    want[:, 1] = -128.0 * 127 * K / 2 ** 20
+    assert torch.equal(out.cpu(), want.half())
+    with pytest.raises(ValueError):
+        fg.linear_int8(torch.zeros(1, 131072, dtype=torch.int8, device=dev), torch.zeros(128, 131072, dtype=torch.int8, device=dev),
+                       torch.zeros(1, 128, dtype=torch.half, device=dev), torch.ones(1, device=dev))
+
+
+def test_rows_do_not_depend_on_their_company(dev):
+    """Exact sums: row i of every path (streaming with each tile height, single CTAs, pairs) has the same bits."""
+    x, w, sx, sw, _ = _data(2600, 8192, 384, 11)
+    xd, wd, sxd, swd = x.to(dev), w.to(dev), sx.to(dev), sw.to(dev)
+    full = torch.empty(2600, 8192, dtype=torch.half, device=dev)
+    fg.linear_int8(xd, wd, full, sxd, swd)
+    for n in (1, 16, 31, 64, 128, 130, 513):
+        out = torch.empty(n, 8192, dtype=torch.half, device=dev)
+        fg.linear_int8(xd[:n], wd, out, sxd[:n], swd)
+        assert torch.equal(out, full[:n]), n
+
+
+@pytest.mark.parametrize("M", [5, 300])
+def test_in_place_residual_and_quantize_int8(M, dev):
+    """Activations from quantize_int8 (fp16 scales); the residual stream updated in place."""
+    g = torch.Generator().manual_seed(2)
+    xf = torch.randn(M, 1024, generator=g).half().to(dev)
+    wf = (torch.randn(512, 1024, generator=g) / 32).half().to(dev)
+    x8, sx = fg.quantize_int8(xf)
+    w8, sw = fg.quantize_int8(wf)
+    res = torch.randn(M, 512, generator=g).half().to(dev)
+    want = ref.linear_int8(x8.cpu(), w8.cpu(), sx.cpu(), sw.cpu(), None, res.cpu())
+    fg.linear_int8(x8, w8, res, sx, sw, residual=res)
+    _check(res, *want)
+
+
+@pytest.mark.parametrize("M", [4, 200])
+def test_gate_from_two_weights(M, dev):
+    g = torch.Generator().manual_seed(8)
+    wg, wu = (torch.randint(-127, 128, (320, 384), generator=g, dtype=torch.int8) for _ in range(2))
+    sg, su, bg, bu = ((torch.rand(320, generator=g) / 100).half() for _ in range(4))
+    x = torch.randint(-127, 128, (M, 384), generator=g, dtype=torch.int8)
+    sx = torch.rand(M, generator=g) / 100
+    w, s, b = (fg.prepack_gate_up(p.to(dev), q.to(dev)) for p, q in ((wg, wu), (sg, su), (bg, bu)))
+    out = torch.empty(M, 320, dtype=torch.half, device=dev)
+    fg.linear_int8(x.to(dev), w, out, sx.to(dev), s, b, act="silu_gate")
+    gate, s1 = ref.linear_int8(x, wg, sx, sg, bg)
+    up, s2 = ref.linear_int8(x, wu, sx, su, bu)
+    _check(out, ref.activation(gate, "silu") * up, (s1 + 1) * (s2 + 1))
+
+
+@pytest.mark.parametrize("M", [8, 100, 160, 2048])
+def test_two_graphs_of_one_stream_side_by_side(M, dev):
+    """Graphs captured on one stream have workspaces of their own: replayed on two streams at once they do not meet."""
+    x, w, sx, sw, _ = _data(M, 4096, 2048, 21)
+    xd, wd, sxd, swd = x.to(dev), w.to(dev), sx.to(dev), sw.to(dev)
+    want = torch.empty(M, 4096, dtype=torch.half, device=dev)
+    fg.linear_int8(xd, wd, want, sxd, swd)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    for _ in range(2):
+        out = torch.zeros(M, 4096, dtype=torch.half, device=dev)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            for _ in range(4):
+                fg.linear_int8(xd, wd, out, sxd, swd)
+        graphs.append(graph)
+        outs.append(out)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s1):
+            graphs[0].replay()
+        with torch.cuda.stream(s2):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+def test_two_streams_and_mixed_with_fp16_linears(dev):
+    """Eager calls on two streams, each between fp16 linears of the same streams (they share the stream's workspace)."""
+    x, w, sx, sw, g = _data(48, 1024, 1024, 31)
+    xd, wd, sxd, swd = x.to(dev), w.to(dev), sx.to(dev), sw.to(dev)
+    xf, wf = torch.randn(48, 1024, generator=g).half().to(dev), (torch.randn(1024, 1024, generator=g) / 32).half().to(dev)
+    want8, want16 = (torch.empty(48, 1024, dtype=torch.half, device=dev) for _ in range(2))
+    fg.linear_int8(xd, wd, want8, sxd, swd)
+    fg.edgemm_m8n128k64x4_bt(xf, wf, want16)
+    torch.cuda.synchronize()
+    got = []
+    for stream in (torch.cuda.Stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                a, b = torch.empty_like(want8), torch.empty_like(want16)
+                fg.linear_int8(xd, wd, a, sxd, swd)
+                fg.edgemm_m8n128k64x4_bt(xf, wf, b)
+                got.append((a, b))
+    torch.cuda.synchronize()
+    for a, b in got:
+        assert torch.equal(a, want8) and torch.equal(b, want16)
+
+
+def test_refusals(dev):
+    x, w = torch.zeros(2, 256, dtype=torch.int8, device=dev), torch.zeros(128, 256, dtype=torch.int8, device=dev)
+    c, s = torch.empty(2, 128, dtype=torch.half, device=dev), torch.ones(2, device=dev)
+    fg.linear_int8(x, w, c, s)
+    fg.linear_int8(x[:0], w, c[:0], s[:0])
+    for bad in (lambda: fg.linear_int8(x[:, :200].contiguous(), w[:, :200].contiguous(), c, s),
+                lambda: fg.linear_int8(x, w[:100], torch.empty(2, 100, dtype=torch.half, device=dev), s),
+                lambda: fg.linear_int8(x, w, c, s, act="relu")):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: fg.linear_int8(x, w, c, s[:1]),
+                lambda: fg.linear_int8(x, w, c, s.double()),
+                lambda: fg.linear_int8(x, w, c.float(), s),
+                lambda: fg.linear_int8(x.half(), w, c, s),
+                lambda: fg.linear_int8(x, w[:, :128].contiguous(), c, s),
+                lambda: fg.linear_int8(x, w, c, s, bias=torch.zeros(64, dtype=torch.half, device=dev)),
+                lambda: fg.linear_int8(x, w, c, s, act="silu_gate")):
+        with pytest.raises(RuntimeError):
+            bad()
+    both = torch.empty(2 * 128 + 128, dtype=torch.half, device=dev)
+    with pytest.raises(ValueError):  # the residual one row further in the same buffer
+        fg.linear_int8(x, w, both[:256].view(2, 128), s, residual=both[128:].view(2, 128))
+    L, ws = capi.lib, torch.empty(capi.workspace_bytes(128), dtype=torch.uint8, device=dev)
+    args = lambda act=0, wsb=ws.numel(): L.fg_linear_w8a8(x.data_ptr(), w.data_ptr(), s.data_ptr(), 1, None, c.data_ptr(), 2, 128, 256, None,
+                                                          None, act, ws.data_ptr(), wsb, ctypes.c_void_p(0))
+    assert args(act=9) == capi.FG_ERR_PLAN and args(wsb=1024) == capi.FG_ERR_WORKSPACE

@@ -1,0 +1,113 @@
+"""What the serving operators refuse before they touch a device, and the host side of the cache (no GPU needed)."""
+import ctypes
+
+import pytest
+import torch
+
+import fastgate_b200 as fg
+from fastgate_b200 import capi
+from fastgate_b200.kvcache import KVCacheInt4, rotation_table
+
+L = capi.lib
+_buf = (ctypes.c_char * 8192)()
+P = (ctypes.addressof(_buf) + 255) // 256 * 256  # aligned host address, never dereferenced
+
+
+def test_norm_arguments():
+    call = lambda x=P, ldx=64, w=P, r=None, ro=None, out=P, i8=0, s=None, M=2, K=64, eps=1e-6: L.fg_add_rmsnorm(x, ldx, w, r, ro, 0, out, i8, s, M, K, eps, None)
+    assert call(x=None) == call(w=None) == call(out=None) == call(i8=1) == call(r=P) == call(ro=P) == capi.FG_ERR_NULL
+    assert call(M=0) == call(K=0) == call(K=60) == call(ldx=32) == call(ldx=68) == call(eps=-1.0) == call(eps=float("nan")) == capi.FG_ERR_SHAPE
+    assert call(x=P + 2) == call(w=P + 8) == call(out=P + 8) == call(r=P + 4, ro=P) == call(i8=1, s=P + 2) == capi.FG_ERR_ALIGN
+
+
+def test_linear_arguments():
+    wsb = capi.workspace_bytes(128)
+    call = lambda x=P, w=P, s=P, c=P, M=1, N=128, K=128, res=None, act=0, ws=P, wsb=wsb: L.fg_linear_w8a8(x, w, s, 1, None, c, M, N, K, None, res, act, ws, wsb, None)
+    assert call(x=None) == call(w=None) == call(s=None) == call(c=None) == capi.FG_ERR_NULL
+    assert call(M=0) == call(N=100) == call(K=64) == call(K=131072) == capi.FG_ERR_SHAPE
+    assert call(act=5) == call(act=-1) == capi.FG_ERR_PLAN
+    assert call(x=P + 8) == call(c=P + 8) == call(res=P + 2) == call(s=P + 2) == capi.FG_ERR_ALIGN
+    assert call(ws=None) == call(ws=P + 16) == call(wsb=4096) == capi.FG_ERR_WORKSPACE
+
+
+def test_cache_arguments():
+    app = lambda k=P, ldk=128, T=1, heads=2, d=64, pages=P, n=4, page=16, slots=P, cs=None, plen=0, pos=None, q=None, ldq=0, qo=None, ldqo=0, qh=0: \
+        L.fg_kv_append_int4(k, ldk, P, 128, T, heads, d, pages, n, page, slots, 1, cs, plen, pos, 1, q, ldq, qo, ldqo, qh, 0, None, None)
+    assert app(k=None) == app(pages=None) == app(slots=None) == app(cs=P) == app(pos=P) == app(q=P, qo=P, qh=1, ldq=64, ldqo=64) == capi.FG_ERR_NULL
+    assert app(T=0) == app(heads=0) == app(d=96) == app(n=0) == app(page=8) == app(page=24) == app(ldk=64) == app(ldk=132) == capi.FG_ERR_SHAPE
+    assert app(qh=3) == app(cs=P, pos=P) == app(cs=P, plen=4, pos=P, q=P, qo=P, qh=2, ldq=64, ldqo=128) == capi.FG_ERR_SHAPE
+    assert app(k=P + 8) == app(pages=P + 8) == app(slots=P + 4) == app(cs=P + 4, plen=4, pos=P) == capi.FG_ERR_ALIGN
+    read = lambda pages=P, T=1, k=P, d=64: L.fg_kv_read_int4(pages, 4, 16, 2, d, P, 1, T, k, P, None, None)
+    assert read(pages=None) == read(k=None) == capi.FG_ERR_NULL
+    assert read(T=0) == read(d=32) == capi.FG_ERR_SHAPE
+    assert read(k=P + 8) == capi.FG_ERR_ALIGN
+    wsb = L.fg_kv_attention_workspace_bytes()
+    att = lambda q=P, ldq=256, T=2, hq=4, hkv=2, d=64, n=4, page=16, ldt=2, width=2, starts=None, batch=2, scale=1.0, ws=P, wsb=wsb: \
+        L.fg_kv_attention_int4(q, ldq, P, 256, T, hq, hkv, d, P, n, page, P, ldt, width, P, starts, batch, scale, None, ws, wsb, None)
+    assert att(q=None) == capi.FG_ERR_NULL
+    assert att(ldq=200) == att(T=3) == att(hq=3) == att(d=80) == att(page=20) == att(ldt=1) == att(width=0) == att(batch=0) == capi.FG_ERR_SHAPE
+    assert att(scale=0.0) == att(scale=float("inf")) == att(width=2 ** 28, ldt=2 ** 28) == capi.FG_ERR_SHAPE
+    assert att(q=P + 8) == att(starts=P + 2) == capi.FG_ERR_ALIGN
+    assert att(ws=None) == att(ws=P + 64) == att(wsb=wsb - 1) == L.fg_kv_attention_workspace_init(None, wsb, None) == capi.FG_ERR_WORKSPACE
+
+
+def test_valid_arguments_stop_at_the_device():
+    """Without a GPU a call that is in order ends with an error, not with a crash."""
+    if torch.cuda.is_available():
+        pytest.skip("a device is there: host addresses would be used")
+    assert L.fg_add_rmsnorm(P, 64, P, None, None, 0, P, 0, None, 2, 64, 1e-6, None) == capi.FG_ERR_NO_DEVICE
+    assert L.fg_linear_w8a8(P, P, P, 1, None, P, 1, 128, 128, None, None, 0, P, capi.workspace_bytes(128), None) == capi.FG_ERR_NO_DEVICE
+    assert L.fg_kv_read_int4(P, 4, 16, 2, 64, P, 1, 1, P, P, None, None) == capi.FG_ERR_NO_DEVICE
+
+
+def test_prepack_of_int8_weights_checks_its_sizes():
+    assert L.fg_prepack_gate_up_w8(None, P, P, 64, 128, None) == capi.FG_ERR_NULL
+    assert L.fg_prepack_gate_up_w8(P, P, P, 65, 128, None) == L.fg_prepack_gate_up_w8(P, P, P, 64, 64, None) == capi.FG_ERR_SHAPE
+
+
+def test_operators_refuse_cpu_tensors():
+    h = torch.zeros(2, 64, dtype=torch.half)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        fg.add_rmsnorm(h, h[0], h.clone())
+    i8 = torch.zeros(2, 128, dtype=torch.int8)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        fg.linear_int8(i8, i8, h, h[:, 0])
+    cache = KVCacheInt4(2, 1, 64, 16, device="cpu")
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        cache.append(h[:, None], h[:, None], torch.arange(2))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        cache.read(torch.arange(2))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        cache.attend(h[:, None], torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32), h[:, None].clone())
+
+
+def test_cache_bookkeeping():
+    cache = KVCacheInt4(6, 2, 128, 32, device="cpu")
+    assert cache.pages.shape == (6, 2, 32 * 136) and cache.pages.dtype == torch.uint8
+    table = torch.tensor([[4, 1], [0, 3]], dtype=torch.int32)
+    got = cache.slots(table, torch.tensor([0, 0, 1, 1, 0]), torch.tensor([0, 33, 31, 32, -1]))
+    assert got.tolist() == [4 * 32, 32 + 1, 31, 3 * 32, -1]
+    for bad in (lambda: KVCacheInt4(2, 1, 100), lambda: KVCacheInt4(2, 1, 64, 8), lambda: KVCacheInt4(0, 1, 64), lambda: KVCacheInt4(2, 0, 64)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_rotation_table_keeps_far_angles():
+    t = rotation_table(200001, 64, device="cpu")
+    assert t.shape == (200001, 64) and t.dtype == torch.float32
+    a = 200000.0 * 10000.0 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64)
+    assert float((t[200000].double() - torch.cat([a.cos(), a.sin()])).abs().max()) <= 2.0 ** -24
+
+
+def test_plan_of_the_streaming_kernel_fits():
+    """Every plan for int8 activations leaves the ring at least two deep, within shared memory and the partial tiles' room."""
+    p = capi.Plan()
+    for M in (1, 16, 17, 32, 33, 64, 65, 128):
+        for N, K in ((128, 128), (4096, 4096), (28672, 8192), (256, 130944), (65536, 384)):
+            for extra in (0, 8192):
+                assert L.fg_plan_w8a8(M, N, K, 148, 232448, extra, ctypes.byref(p)) == capi.FG_OK
+                assert p.m_tile >= min(M, 128) and p.passes == 1 and p.stages >= 2 and p.smem_bytes <= 232448
+                assert p.k_per_stage % 128 == 0 and p.k_blocks * p.k_per_stage >= K > (p.k_blocks - 1) * p.k_per_stage
+                assert 1 <= p.grid <= 148 and p.grid * 2 * p.m_tile * 128 * 4 <= 256 * 2 * 64 * 128 * 4
+                assert p.smem_bytes >= 1024 + p.stages * ((p.k_per_stage // 128) * (16384 + 128 * p.m_tile) + 16) + 64 + extra
+    assert L.fg_plan_w8a8(1, 100, 128, 148, 232448, 0, ctypes.byref(p)) == capi.FG_ERR_SHAPE
