@@ -27,7 +27,7 @@ NVCC_FLAGS = [
 # translation units of libfastgate_b200.so
 LIB_SOURCES = ("fg_capi.cu", "fg_plan.cpp", "fg_norm.cu", "fg_linear8.cu", "fg_kv4.cu", "fg_attn4.cu")
 # translation units of the pybind extension
-EXT_SOURCES = ("fg_torch.cpp", "fg_torch_serving.cpp")
+EXT_SOURCES = ("fg_torch.cpp", "fg_torch_serving.cpp", "fg_torch_graph.cpp")
 
 
 def _newer(target: str, sources: list[str]) -> bool:

@@ -17,17 +17,19 @@
 //     movmatrix makes the second product's operand; nothing goes through shared memory but the cache itself.
 //     (tcgen05.mma takes its operands from shared memory: the codes would have to be written back there as fp16, four
 //     times the bytes that came in.)
-//   - The softmax's running maximum moves only when a score exceeds it by more than 2^8 (a warp vote per 16 rows instead
+//   - The softmax's running maximum moves only when a weight exceeds it by more than 2^8 (a warp vote per 32 rows instead
 //     of a reduction); weights then stay below 2^8 and exact sums are unchanged, since every term uses the same m.
 //     The maximum is taken over log2(p_t sv_t), the weight that is rounded to fp16: its relative error is 2^-11 whatever
 //     the scale of the values.
 //
-// Each warp streams its own blocks of 16 rows through its own ring (bulk copies by lane 0, one mbarrier per slot), so no
-// warp waits for another inside a segment.  The rows of all (sequence, head, query tile) items form one list of 64-row
+// Each warp streams its own slots of four blocks through its own ring (bulk copies, one mbarrier per slot), so no
+// warp waits for another inside a segment.  The rows of all (sequence, head, query tile) items form one list of 256-row
 // units that is dealt out evenly to the CTAs whatever the lengths; an item that several CTAs share is joined by the last of
 // them to finish, in CTA order (deterministic), from partial sums in the workspace.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "../../include/fastgate_b200.h"
 #include "fg_host.h"
@@ -38,19 +40,30 @@ namespace {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
-constexpr int kAttnStages = 4;             // ring slots of a warp
-constexpr int kUnitRows = kAttnWarps * kKvBlock;
+constexpr int kPairRows = 2 * kKvBlock;       // rows that one step of the softmax takes
+constexpr int kSlotBlocks = 4;                // blocks of a ring slot
+constexpr int kSlotRows = kSlotBlocks * kKvBlock;
+constexpr int kUnitRows = kAttnWarps * kSlotRows;
 constexpr int kAttnMaxGrid = 1024;
-constexpr int kAttnMinUnits = 4;           // units a CTA gets at least, so that joining stays cheap
-constexpr float kLazyMax = 8.f;            // log2 of how far a weight may exceed the running maximum
+constexpr float kLazyMax = 8.f;               // log2 of how far a weight may exceed the running maximum
+constexpr float kNoMax = -1e30f;              // stands for the maximum of no rows (scores stay far above it)
+constexpr float kMaxScale = 1048576.f;        // largest softmax scale: |scores| < 2^20 * 128 * 2^36
 constexpr unsigned long long kAttnWaitNs = 2000000000ull;
-constexpr int kStatusAttnTimeout = 6;      // FG_ERR_TIMEOUT
+constexpr int kStatusAttnTimeout = 6;         // FG_ERR_TIMEOUT
 
 // Workspace: [0,256) header, kAttnMaxGrid tickets (zero between launches), then two partials per CTA.
 constexpr size_t kAttnTicketsOffset = 256;
 constexpr size_t kAttnPartialsOffset = kAttnTicketsOffset + kAttnMaxGrid * 4;
-constexpr int kAttnMaxCols = 16;
 __host__ __device__ constexpr int partial_floats(int d, int cols) { return cols * (d + 4); }  // [cols][d] sums, [cols] maxima, [cols] norms, padding
+__host__ __device__ constexpr int attn_stages(int d) { return (d == 128 ? 8 : 12) / kSlotBlocks; }  // ring slots of a warp
+__host__ __device__ constexpr int attn_slot_bytes(int d, int cols) {                          // a warp's sums are parked in the slot it has emptied last
+  return kSlotBlocks * kv_block_bytes(d) > cols * d * 4 ? kSlotBlocks * kv_block_bytes(d) : cols * d * 4;
+}
+__host__ __device__ constexpr int attn_smem_bytes(int d, int cols) { return kAttnWarps * attn_stages(d) * attn_slot_bytes(d, cols); }
+// What the registers allow without spilling: 165 with eight columns, 255 with sixteen.  (Measured, 64 sequences of up to 8000
+// rows, eight columns, two / three / four CTAs: 119 / 86 / 88 us; 24 x 3000 rows of 64 channels, sixteen columns: 20.6 / 22.9 / 28.4.)
+__host__ __device__ constexpr int attn_ctas_per_sm(int cols) { return cols == 8 ? 3 : 2; }
+constexpr int kAttnMaxCols = 16;
 
 struct AttnParams {
   const __half* q;        // [tokens, q_heads, D], token stride ldq
@@ -82,6 +95,11 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+__device__ __forceinline__ uint32_t add_release(unsigned int* p, unsigned int v) {
+  uint32_t r;
+  asm volatile("atom.add.release.gpu.global.u32 %0, [%1], %2;" : "=r"(r) : "l"(p), "r"(v) : "memory");
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -92,25 +110,35 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// Words of a shared-memory row (ordinary loads: the compiler may place them).
 template <int BYTES>
-__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[BYTES / 4]) {
-  if constexpr (BYTES == 16) lds_v4(addr, w[0], w[1], w[2], w[3]);
-  else if constexpr (BYTES == 8) lds_v2(addr, w[0], w[1]);
-  else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[BYTES / 4]) {
+  if constexpr (BYTES == 16) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (BYTES == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
 }
-__device__ __forceinline__ float2 lds_half2(uint32_t addr) {
-  uint32_t w;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(addr));
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+__device__ __forceinline__ float2 lds_half2(const uint8_t* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
+// D(16x8, f32) = A(16x16, f16, row) B(16x8, f16, col) + C
+__device__ __forceinline__ void mma_codes(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                          float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 // What of the work list belongs to sequence b.
 struct Sequence {
-  int len;       // rows that its queries may see at most
-  int q0, nq;    // its query tokens
-  int tiles;     // query tiles per key/value head
-  int units;     // units per item, at least one
-  __device__ long long total(int kv_heads) const { return static_cast<long long>(tiles) * kv_heads * units; }
+  int len;         // its rows in the cache
+  int q0, nq;      // its query tokens
+  uint32_t tiles;  // query tiles per key/value head
+  uint32_t units;  // units per item, at least one
+  __device__ uint32_t total(int kv_heads) const { return tiles * kv_heads * units; }  // < 2^31: the host has checked
 };
 
 template <int COLS>
@@ -118,8 +146,7 @@ __device__ __forceinline__ Sequence sequence(const AttnParams& p, int b, bool re
   Sequence s;
   bool bad = false;
   s.len = p.lens[b];
-  const long long room = static_cast<long long>(p.table_width) * p.kv.page_size;
-  if (s.len < 0 || s.len > room) {
+  if (s.len < 0 || s.len > p.table_width * p.kv.page_size) {
     bad = true;
     s.len = 0;  // its outputs become zeros
   }
@@ -130,65 +157,87 @@ __device__ __forceinline__ Sequence sequence(const AttnParams& p, int b, bool re
     s.q0 = s.nq = 0;  // nothing is read or written for it
   }
   if (bad && report && p.status != nullptr) atomicExch(p.status, kStatusIndex);
-  s.tiles = static_cast<int>((static_cast<long long>(s.nq) * p.group + COLS - 1) / COLS);
+  s.tiles = (static_cast<uint32_t>(s.nq) * p.group + COLS - 1) / COLS;
   s.units = s.len > 0 ? (s.len + kUnitRows - 1) / kUnitRows : 1;
   return s;
 }
 
+// A place in the work list.
+struct Walk {
+  int b;            // sequence
+  uint32_t before;  // units before it
+  Sequence sq;
+};
+struct Segment {
+  uint32_t item_u0;     // first unit of the item
+  int first, len;       // units of the item
+  int head, tile;
+};
+
+// An item of which this CTA has left a partial: joined at the CTA's end if it was the last to leave one.
+struct Pending {
+  uint32_t first, parts;  // the CTAs that share the item
+  uint32_t first_slot;    // which of its two partials the first one's is
+  uint32_t ticket;        // how many had left theirs before
+  int cols, tile, head, q0;
+};
+
 template <int D, int NQ>
-__global__ void __launch_bounds__(kAttnThreads, NQ == 1 ? 4 : 3) fg_kv_attention_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kAttnThreads, attn_ctas_per_sm(8 * NQ)) fg_kv_attention_kernel(const AttnParams p) {
   constexpr int COLS = 8 * NQ;          // query columns of an item
   constexpr int KW = D / 32;            // 32-bit words of a key row per lane
   constexpr int VW = D / 64;            // 32-bit words of a value row per lane
   constexpr int MT = D / 16;            // 16-channel accumulator tiles
   constexpr int SB = kv_block_bytes(D);
-  constexpr int kRing = kAttnStages * SB;
-  constexpr int kWarpBytes = (kRing > COLS * (D + 4) * 4 ? kRing : COLS * (D + 4) * 4);  // a warp's sums are parked in its ring
+  constexpr int S = attn_stages(D);
+  constexpr int kSlot = attn_slot_bytes(D, COLS);
+  constexpr uint32_t kNoBlock = 0xffffffffu, kSlotMask = (1u << kSlotBlocks) - 1;
+  constexpr int kSet = 32 / kSlotBlocks;  // slots whose blocks the lanes of a warp hold
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) unsigned long long bars[kAttnWarps * kAttnStages];
-  __shared__ long long scan[kAttnWarps + 1];
-  __shared__ long long start_before;
+  __shared__ __align__(8) unsigned long long bars[kAttnWarps * S];
+  __shared__ uint32_t scan[kAttnWarps], start_before;
   __shared__ int start_b;
-  __shared__ unsigned int ticket;
+  __shared__ Pending pending[2];
+  __shared__ float warp_max[kAttnWarps][COLS], warp_norm[kAttnWarps][COLS];
+  __shared__ const float* warp_sums[kAttnWarps];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  uint8_t* my_smem = smem + warp * kWarpBytes;
-  const uint32_t ring = smem_u32(my_smem);
-  const uint32_t bar = smem_u32(bars + warp * kAttnStages);
-  if (lane < kAttnStages) mbar_init(bar + 8 * lane, 1);
+  uint8_t* ring = smem + warp * (S * kSlot);
+  const uint32_t ring_u32 = smem_u32(ring);
+  const uint32_t bar = smem_u32(bars + warp * S);
+  if (lane < S) mbar_init(bar + 8 * lane, 1);
   fence_mbar_init();
   fence_proxy_async();
   griddep_launch_dependents();
   griddep_wait();
 
-  // ---- this CTA's share [ub, ue) of the work list ----
+  // ---- this CTA's share [ub, ue) of the work list: equal runs of `chunk` units ----
+  const int kv_heads = p.kv.heads;
   const int per = (p.batch + kAttnThreads - 1) / kAttnThreads;
   const int b_lo = min(p.batch, tid * per), b_hi = min(p.batch, b_lo + per);
-  long long mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += sequence<COLS>(p, b, blockIdx.x == 0).total(p.kv.heads);
-  long long incl = mine;
+  uint32_t mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += sequence<COLS>(p, b, blockIdx.x == 0).total(kv_heads);
+  uint32_t incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, off);
+    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, off);
     if (lane >= off) incl += v;
   }
   if (lane == 31) scan[warp] = incl;
   __syncthreads();
-  long long before = incl - mine, total = 0;
+  uint32_t before = incl - mine, total = 0;
 #pragma unroll
   for (int w = 0; w < kAttnWarps; ++w) {
     if (w < warp) before += scan[w];
     total += scan[w];
   }
-  const long long want = (total + kAttnMinUnits - 1) / kAttnMinUnits;
-  const long long G = want < gridDim.x ? want : gridDim.x;
-  if (static_cast<long long>(blockIdx.x) >= G) return;
-  const long long cta = blockIdx.x;
-  const long long ub = cta * total / G, ue = (cta + 1) * total / G;
-  if (mine > 0 && ub >= before && ub < before + mine) {
+  const uint32_t chunk = (total + gridDim.x - 1) / gridDim.x;
+  const uint32_t cta = blockIdx.x, ub = cta * chunk, ue = min(total, ub + chunk);
+  if (ub >= total) return;
+  if (ub >= before && ub - before < mine) {
     int b = b_lo;
     for (;; ++b) {
-      const long long t = sequence<COLS>(p, b, false).total(p.kv.heads);
+      const uint32_t t = sequence<COLS>(p, b, false).total(kv_heads);
       if (ub < before + t) break;
       before += t;
     }
@@ -196,54 +245,155 @@ __global__ void __launch_bounds__(kAttnThreads, NQ == 1 ? 4 : 3) fg_kv_attention
     start_before = before;
   }
   __syncthreads();
-  int b = start_b;
-  long long b_before = start_before;  // units before sequence b
-  Sequence sq = sequence<COLS>(p, b, false);
-
-  uint32_t phase = 0;  // one bit per ring slot
-  bool dead = false;
-  long long u = ub;
-  while (u < ue) {
-    while (u >= b_before + sq.total(p.kv.heads)) {
-      b_before += sq.total(p.kv.heads);
-      sq = sequence<COLS>(p, ++b, false);
+  auto settle = [&](Walk& w, uint32_t u) {  // to the sequence that holds unit u
+    while (u >= w.before + w.sq.total(kv_heads)) {
+      w.before += w.sq.total(kv_heads);
+      w.sq = sequence<COLS>(p, ++w.b, false);
     }
-    // ---- the segment: units [seg0, seg0 + seg_len) of item (b, head, tile) ----
-    const long long item = (u - b_before) / sq.units;
-    const long long item_u0 = b_before + item * sq.units;
-    const int seg0 = static_cast<int>(u - item_u0);
-    const int seg_len = static_cast<int>(min(static_cast<long long>(sq.units - seg0), ue - u));
-    const int head = static_cast<int>(item / sq.tiles), tile = static_cast<int>(item - static_cast<long long>(head) * sq.tiles);
-    const int cols = min(COLS, sq.nq * p.group - tile * COLS);
+  };
+  auto segment_at = [&](const Walk& w, uint32_t u) {  // from unit u to the end of its item or of the share
+    Segment s;
+    const uint32_t item = (u - w.before) / w.sq.units;
+    s.item_u0 = w.before + item * w.sq.units;
+    s.first = static_cast<int>(u - s.item_u0);
+    s.len = static_cast<int>(min(w.sq.units - s.first, ue - u));
+    s.head = static_cast<int>(item / w.sq.tiles);
+    s.tile = static_cast<int>(item - s.head * w.sq.tiles);
+    return s;
+  };
+  // slots that this warp takes of a segment: warp, warp + 4, ... counted from its first row
+  auto slots_of = [&](const Walk& w, const Segment& s) {
+    const int first = s.first * kAttnWarps + warp, end = min((w.sq.len + kSlotRows - 1) / kSlotRows, (s.first + s.len) * kAttnWarps);
+    return end > first ? (end - first + kAttnWarps - 1) / kAttnWarps : 0;
+  };
 
-    // ---- queries into fragments, their sums, the last row that each column sees ----
-    uint32_t qf[NQ][KW][4];
-    float qs[NQ][2];
-    int limit[NQ][2], min_limit = 0x7fffffff;
+  // ---- copies: a cursor that runs up to S slots ahead of the rows being used, across segments ----
+  const int blocks_per_page = p.kv.page_size / kKvBlock;
+  Walk cw = {start_b, start_before, sequence<COLS>(p, start_b, false)};
+  uint32_t cu = ub;                  // where the cursor's segment begins
+  int c_slots = 0, c_next = 0;       // its slots of this warp, and the next one to be copied
+  int c_first = 0, c_head = 0, c_slot = 0;
+  uint32_t now_at, now_bytes, now_none, next_at, next_bytes, next_none;
+  uint32_t gone = 0;                 // a bit per block of the ring: those that are not there
+  // Lane kSlotBlocks i + k holds block k of the i-th of kSet slots: its number, and how many bytes to copy from it (neighbouring blocks
+  // of a slot that lie side by side in the pool are one copy).  `none`: which of the 32 are absent.
+  auto fetch = [&](int set, uint32_t& at, uint32_t& bytes, uint32_t& none) {
+    const int i = kSet * set + lane / kSlotBlocks, blk = (c_first + i * kAttnWarps) * kSlotBlocks + lane % kSlotBlocks;
+    at = kNoBlock;
+    if (i < c_slots && blk * kKvBlock < cw.sq.len) {
+      const int nth = blk / blocks_per_page, page = __ldg(p.table + static_cast<long long>(cw.b) * p.ldt + nth);
+      if (page >= 0 && page < p.kv.pages)
+        at = (static_cast<uint32_t>(page) * kv_heads + c_head) * blocks_per_page + (blk - nth * blocks_per_page);
+      else if (p.status != nullptr)
+        atomicExch(p.status, kStatusIndex);
+    }
+    const uint32_t left = __shfl_up_sync(0xffffffffu, at, 1);
+    const bool follows = lane % kSlotBlocks != 0 && at != kNoBlock && left != kNoBlock && at == left + 1;
+    const uint32_t chain = __ballot_sync(0xffffffffu, follows);
+    none = __ballot_sync(0xffffffffu, at == kNoBlock);
+    const int run = lane == 31 ? 1 : __ffs(~(chain >> (lane + 1)));  // 1 + the blocks that follow
+    bytes = at != kNoBlock && !follows ? run * SB : 0;
+  };
+  auto open = [&](uint32_t u) {  // the cursor enters the segment that begins at u, or the first after it with rows for this warp
+    for (cu = u; cu < ue;) {
+      settle(cw, cu);
+      const Segment s = segment_at(cw, cu);
+      c_slots = slots_of(cw, s);
+      c_next = 0;
+      cu += s.len;
+      if (c_slots > 0) {
+        c_first = s.first * kAttnWarps + warp;
+        c_head = s.head;
+        fetch(0, now_at, now_bytes, now_none);
+        if (c_slots > kSet) fetch(1, next_at, next_bytes, next_none);
+        return;
+      }
+    }
+    c_slots = c_next = 0;
+  };
+  auto copy_next = [&]() {  // whole warp: the next slot of the stream into the ring
+    if (c_next == c_slots) {
+      if (c_slots == 0 && cu >= ue) return;
+      open(cu);
+      if (c_slots == 0) return;
+    }
+    const int i = c_next % kSet;
+    const uint32_t missing = (now_none >> (kSlotBlocks * i)) & kSlotMask;
+    gone = (gone & ~(kSlotMask << (kSlotBlocks * c_slot))) | (missing << (kSlotBlocks * c_slot));
+    if (lane / kSlotBlocks == i) {
+      const uint32_t full = bar + 8 * c_slot;
+      if (lane % kSlotBlocks == 0) mbar_arrive_expect_tx(full, SB * (kSlotBlocks - __popc(missing)));
+      if (now_bytes != 0)
+        bulk_load(ring_u32 + c_slot * kSlot + (lane % kSlotBlocks) * SB, p.kv.base + static_cast<size_t>(now_at) * SB, now_bytes, full);
+    }
+    __syncwarp();
+    c_slot = c_slot + 1 == S ? 0 : c_slot + 1;
+    ++c_next;
+    if (c_next % kSet == 0 && c_next < c_slots) {
+      now_at = next_at;
+      now_bytes = next_bytes;
+      now_none = next_none;
+      if (c_next + kSet < c_slots) fetch(c_next / kSet + 1, next_at, next_bytes, next_none);
+    }
+  };
+  // Output: a thread has four channels of every (kAttnThreads / (D / 4))th column.
+  constexpr int TPC = D / 4;
+  constexpr uint32_t kJoin = 8;
+  const int d4 = (tid % TPC) * 4;
+  auto write_out = [&](int flat, int head, int q0, float4 v, float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
+    const __half2 h0 = __floats2half2_rn(v.x * inv, v.y * inv), h1 = __floats2half2_rn(v.z * inv, v.w * inv);
+    *reinterpret_cast<uint2*>(p.out + static_cast<long long>(q0 + flat / p.group) * p.ldo +
+                              static_cast<long long>(head * p.group + flat % p.group) * D + d4) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+  };
+
+  // ---- queries: 16-byte pieces of a segment's columns, fetched ahead of their use ----
+  uint4 raw[NQ][KW];
+  auto load_queries = [&](const Sequence& sq, const Segment& seg) {
+    const int cols = min(COLS, sq.nq * p.group - seg.tile * COLS);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const int col = n * 8 + g;
+      const int col = n * 8 + g, flat = seg.tile * COLS + col;
+      const __half* src = p.q + static_cast<long long>(sq.q0 + flat / p.group) * p.ldq +
+                          static_cast<long long>(seg.head * p.group + flat % p.group) * D + c * (8 * KW);
+#pragma unroll
+      for (int i = 0; i < KW; ++i) raw[n][i] = col < cols ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  Walk w = cw;
+  settle(w, ub);
+  Segment seg = segment_at(w, ub);
+  load_queries(w.sq, seg);
+  open(ub);
+  for (int i = 0; i < S; ++i) copy_next();
+
+  uint32_t phase = 0;  // one bit per ring slot
+  int slot = 0, n_pending = 0;
+  bool dead = false;
+  for (uint32_t u = ub; u < ue;) {
+    const Sequence sq = w.sq;
+    const int head = seg.head, tile = seg.tile;
+    const int cols = min(COLS, sq.nq * p.group - tile * COLS);
+    const int n_slots = dead ? 0 : slots_of(w, seg);
+
+    // ---- queries as fragments, their sums, the last row that each column sees ----
+    uint32_t qf[NQ][KW][4];
+    float qs[NQ][2];
+    int limit[NQ][2];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
       float sum = 0.f;
-      uint4 raw[KW];
 #pragma unroll
-      for (int w = 0; w < KW; ++w) raw[w] = make_uint4(0, 0, 0, 0);
-      if (col < cols) {
-        const int flat = tile * COLS + col;
-        const __half* src = p.q + static_cast<long long>(sq.q0 + flat / p.group) * p.ldq +
-                            static_cast<long long>(head * p.group + flat % p.group) * D + c * (8 * KW);
-#pragma unroll
-        for (int w = 0; w < KW; ++w) raw[w] = *reinterpret_cast<const uint4*>(src + 8 * w);
-      }
-#pragma unroll
-      for (int w = 0; w < KW; ++w) {
+      for (int i = 0; i < KW; ++i) {
         // channels (0,4), (2,6) meet the low nibbles' pairs, (1,5), (3,7) the high ones'
-        qf[n][w][0] = prmt(raw[w].x, raw[w].z, 0x5410);
-        qf[n][w][1] = prmt(raw[w].y, raw[w].w, 0x5410);
-        qf[n][w][2] = prmt(raw[w].x, raw[w].z, 0x7632);
-        qf[n][w][3] = prmt(raw[w].y, raw[w].w, 0x7632);
+        qf[n][i][0] = prmt(raw[n][i].x, raw[n][i].z, 0x5410);
+        qf[n][i][1] = prmt(raw[n][i].y, raw[n][i].w, 0x5410);
+        qf[n][i][2] = prmt(raw[n][i].x, raw[n][i].z, 0x7632);
+        qf[n][i][3] = prmt(raw[n][i].y, raw[n][i].w, 0x7632);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qf[n][w][i]));
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qf[n][i][k]));
           sum += f.x + f.y;
         }
       }
@@ -256,14 +406,14 @@ __global__ void __launch_bounds__(kAttnThreads, NQ == 1 ? 4 : 3) fg_kv_attention
         limit[n][i] = my < cols ? sq.len - sq.nq + (tile * COLS + my) / p.group : sq.len - 1;
       }
     }
-    min_limit = min(sq.len - 1, sq.len - sq.nq + (tile * COLS) / p.group);  // column 0 sees least
+    const int min_limit = sq.len - sq.nq + (tile * COLS) / p.group;  // column 0 sees least
 
     float oacc[NQ][MT][4], mref[NQ][2], lsum[NQ][2], zsum[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        mref[n][i] = -INFINITY;
+        mref[n][i] = 0.f;
         lsum[n][i] = zsum[n][i] = 0.f;
       }
 #pragma unroll
@@ -272,126 +422,89 @@ __global__ void __launch_bounds__(kAttnThreads, NQ == 1 ? 4 : 3) fg_kv_attention
         for (int i = 0; i < 4; ++i) oacc[n][t][i] = 0.f;
     }
 
-    // ---- this warp's blocks: seg0 * 4 + warp, + 4, ... ----
-    const int blocks_per_page = p.kv.page_size / kKvBlock;
-    const int all_blocks = (sq.len + kKvBlock - 1) / kKvBlock;
-    const int blk0 = seg0 * kAttnWarps + warp;
-    const int blk_end = min(all_blocks, (seg0 + seg_len) * kAttnWarps);
-    const int n_blk = blk_end > blk0 && !dead ? (blk_end - blk0 + kAttnWarps - 1) / kAttnWarps : 0;
-    const int* trow = p.table + static_cast<long long>(b) * p.ldt;
-    // lane i holds the page of this warp's block 32 k + i; `pages_next` the 32 after those
-    auto fetch_pages = [&](int k) {
-      const int blk = blk0 + (32 * k + lane) * kAttnWarps;
-      int page = -1;
-      if (blk < blk_end) {
-        page = __ldg(trow + blk / blocks_per_page);
-        if (page < 0 || page >= p.kv.pages) {
-          if (p.status != nullptr) atomicExch(p.status, kStatusIndex);
-          page = -1;
-        }
-      }
-      return page;
-    };
-    int pages_now = fetch_pages(0), pages_next = fetch_pages(1);
-    uint32_t skipped = 0;  // bit s: the block in slot s has no page and is left out
-    auto issue = [&](int j) {  // whole warp; block j of this warp into slot j % stages
-      if (j >= n_blk) return;
-      const int page = __shfl_sync(0xffffffffu, (j & 32) ? pages_next : pages_now, j & 31);
-      const int s = j % kAttnStages;
-      if (page < 0) {
-        skipped |= 1u << s;
-        return;
-      }
-      skipped &= ~(1u << s);
-      if (lane == 0) {
-        const int blk = blk0 + j * kAttnWarps;
-        mbar_arrive_expect_tx(bar + 8 * s, SB);
-        bulk_load(ring + s * SB, kv_block_ptr(p.kv, D, page, head, blk % blocks_per_page), SB, bar + 8 * s);
-      }
-    };
-    for (int j = 0; j < kAttnStages; ++j) issue(j);
-
-    // key row g of a 16-row operand is row kmap(g) of the block's half: rows 2i and 2i + 1 of an operand then lie in
-    // different halves of the shared-memory banks
+    // Operand row g of a 16-row block is its row ka, operand row g + 8 its row ka + 8: rows 2i and 2i + 1 of an operand then
+    // lie in different halves of the shared-memory banks.
     const int ka = (g & 1) ? 4 + ((g >> 1) ^ 1) : g >> 1;
     const int v0 = c, v1 = 4 + (c ^ 1);
-    for (int j = 0; j < n_blk && !dead; ++j) {
-      const int s = j % kAttnStages;
-      const bool skip = (skipped >> s) & 1u;
-      if (!skip) {
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar + 8 * s, (phase >> s) & 1u, kAttnWaitNs))) {
-          dead = true;
-          if (lane == 0 && p.status != nullptr) atomicExch(p.status, kStatusAttnTimeout);
-          break;
-        }
-        phase ^= 1u << s;
-        const uint32_t base = ring + s * SB;
-        const int row0 = (blk0 + j * kAttnWarps) * kKvBlock;
-
+    bool fresh = true;  // no rows yet: the first ones set the maximum, whatever its size
+    // Two blocks.  MASKED: some column does not see all of their rows, or a block is absent.
+    auto consume = [&](const uint8_t* base, int row0, uint32_t absent, auto masked_tag) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
+      float t[2][NQ][4];         // log2 of the weights over the values' scales, less the running maximum
+      float sv[2][2], lv[2][2];  // the value rows' scale and low end
+      bool up = fresh;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* blk = base + h * SB;
         // S^T = K Q^T on the codes
         uint32_t wa[KW], wb[KW];
-        lds_words<4 * KW>(base + kv_codes_offset(D, 0, ka) + c * (4 * KW), wa);
-        lds_words<4 * KW>(base + kv_codes_offset(D, 0, ka + 8) + c * (4 * KW), wb);
+        lds_words<4 * KW>(blk + kv_codes_offset(D, 0, ka) + c * (4 * KW), wa);
+        lds_words<4 * KW>(blk + kv_codes_offset(D, 0, ka + 8) + c * (4 * KW), wb);
         float slo[NQ][4], shi[NQ][4];
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) slo[n][i] = shi[n][i] = 0.f;
-#pragma unroll
-        for (int w = 0; w < KW; ++w) {
-          const uint32_t xa = wa[w] >> 8, xb = wb[w] >> 8;
+        for (int i = 0; i < KW; ++i) {
+          const uint32_t xa = wa[i] >> 8, xb = wb[i] >> 8;
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
-            mma_16816(slo[n], wa[w] & 0x000F000Fu, wb[w] & 0x000F000Fu, xa & 0x000F000Fu, xb & 0x000F000Fu, qf[n][w][0], qf[n][w][1]);
-            mma_16816(shi[n], wa[w] & 0x00F000F0u, wb[w] & 0x00F000F0u, xa & 0x00F000F0u, xb & 0x00F000F0u, qf[n][w][2], qf[n][w][3]);
+            float *l = slo[n], *u = shi[n];
+            mma_codes(slo[n], wa[i] & 0x000F000Fu, wb[i] & 0x000F000Fu, xa & 0x000F000Fu, xb & 0x000F000Fu, qf[n][i][0], qf[n][i][1],
+                      i ? l[0] : 0.f, i ? l[1] : 0.f, i ? l[2] : 0.f, i ? l[3] : 0.f);
+            mma_codes(shi[n], wa[i] & 0x00F000F0u, wb[i] & 0x00F000F0u, xa & 0x00F000F0u, xb & 0x00F000F0u, qf[n][i][2], qf[n][i][3],
+                      i ? u[0] : 0.f, i ? u[1] : 0.f, i ? u[2] : 0.f, i ? u[3] : 0.f);
           }
         }
-
-        float2 kp[2], vp[2];  // (scale, low) of rows ka and ka + 8
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          kp[i] = lds_half2(base + kv_params_offset(D, 0, ka + 8 * i));
-          vp[i] = lds_half2(base + kv_params_offset(D, 1, ka + 8 * i));
-        }
-        const bool masked = row0 + kKvBlock - 1 > min_limit;
-        float sk[2], lv[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          sk[i] = kp[i].x * (p.scale_log2 * 16777216.f);
-          lv[i] = lg2(fmaxf(vp[i].x, 5.9604644775390625e-8f));
-        }
-        float s2[NQ][4];  // log2 of the weights before the values' scales
-        bool up = false;
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = i >> 1, q = i & 1;
-            s2[n][i] = fmaf(fmaf(shi[n][i], 0.0625f, slo[n][i]), sk[r], kp[r].y * qs[n][q]);
-            if (masked && row0 + ka + 8 * r > limit[n][q]) s2[n][i] = -INFINITY;
-            up |= s2[n][i] + lv[r] > mref[n][q] + kLazyMax;
-          }
-        if (__any_sync(0xffffffffu, up)) {
-          // a new maximum: the largest of the old one and this block's, and everything so far brought to it
+        for (int r = 0; r < 2; ++r) {
+          const float2 kp = lds_half2(blk + kv_params_offset(D, 0, ka + 8 * r)), vp = lds_half2(blk + kv_params_offset(D, 1, ka + 8 * r));
+          const float sk = kp.x * (p.scale_log2 * 16777216.f);
+          sv[h][r] = vp.x;
+          lv[h][r] = vp.y;
+          const float most = kLazyMax - lg2(fmaxf(vp.x, 5.9604644775390625e-8f));  // weight * scale <= 2^kLazyMax
 #pragma unroll
           for (int n = 0; n < NQ; ++n)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-              float m = fmaxf(s2[n][q] + lv[0], s2[n][2 + q] + lv[1]);
-#pragma unroll
-              for (int off = 4; off <= 16; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-              m = fmaxf(m, mref[n][q]);
-              const float f = m == -INFINITY ? 1.f : ex2(mref[n][q] - m);
-              mref[n][q] = m;
-              lsum[n][q] *= f;
-              zsum[n][q] *= f;
-#pragma unroll
-              for (int t = 0; t < MT; ++t) {
-                oacc[n][t][q] *= f;
-                oacc[n][t][2 + q] *= f;
-              }
+              float v = fmaf(fmaf(shi[n][2 * r + q], 0.0625f, slo[n][2 * r + q]), sk, fmaf(kp.y, qs[n][q], -mref[n][q]));
+              if (MASKED && (row0 + 16 * h + ka + 8 * r > limit[n][q] || ((absent >> h) & 1u))) v = -INFINITY;
+              t[h][n][2 * r + q] = v;
+              up |= v > most;
             }
         }
+      }
+      if (__any_sync(0xffffffffu, up)) {
+        // a new maximum: the largest of the old one and these rows', and everything so far brought to it
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float m = fresh ? -INFINITY : 0.f;  // relative to the old one
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) m = fmaxf(m, t[h][n][2 * r + q] + lg2(fmaxf(sv[h][r], 5.9604644775390625e-8f)));
+#pragma unroll
+            for (int off = 4; off <= 16; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+            if (m == -INFINITY) m = 0.f;  // a column that sees none of them (nor, then, any later row)
+            const float f = fresh ? 1.f : ex2(-m);
+            mref[n][q] += m;
+            lsum[n][q] *= f;
+            zsum[n][q] *= f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              t[h][n][q] -= m;
+              t[h][n][2 + q] -= m;
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              oacc[n][i][q] *= f;
+              oacc[n][i][2 + q] *= f;
+            }
+          }
+        if (absent != 3u) fresh = false;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* blk = base + h * SB;
         uint32_t pb[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -399,55 +512,79 @@ __global__ void __launch_bounds__(kAttnThreads, NQ == 1 ? 4 : 3) fg_kv_attention
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = i >> 1, q = i & 1;
-            const float m = mref[n][q] == -INFINITY ? 0.f : mref[n][q];
-            const float e = ex2(s2[n][i] - m);
+            const float e = ex2(t[h][n][i]);
             lsum[n][q] += e;
-            if (masked && s2[n][i] == -INFINITY) {
+            if (MASKED && t[h][n][i] == -INFINITY) {
               wgt[i] = 0.f;  // whatever the row's parameters hold
             } else {
-              zsum[n][q] = fmaf(e, vp[r].y, zsum[n][q]);
-              wgt[i] = e * vp[r].x;
+              zsum[n][q] = fmaf(e, lv[h][r], zsum[n][q]);
+              wgt[i] = e * sv[h][r];
             }
           }
           const __half2 h0 = __floats2half2_rn(wgt[0], wgt[1]), h1 = __floats2half2_rn(wgt[2], wgt[3]);
           pb[n][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&h0));
           pb[n][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&h1));
         }
-
         // O^T += V^T P^T on the codes: lane g owns channels 8 VW g.., operand columns are rows (v0, v1) and (v0, v1) + 8
         uint32_t r0[VW], r1[VW], r2[VW], r3[VW];
-        lds_words<4 * VW>(base + kv_codes_offset(D, 1, v0) + g * (4 * VW), r0);
-        lds_words<4 * VW>(base + kv_codes_offset(D, 1, v1) + g * (4 * VW), r1);
-        lds_words<4 * VW>(base + kv_codes_offset(D, 1, v0 + 8) + g * (4 * VW), r2);
-        lds_words<4 * VW>(base + kv_codes_offset(D, 1, v1 + 8) + g * (4 * VW), r3);
+        lds_words<4 * VW>(blk + kv_codes_offset(D, 1, v0) + g * (4 * VW), r0);
+        lds_words<4 * VW>(blk + kv_codes_offset(D, 1, v1) + g * (4 * VW), r1);
+        lds_words<4 * VW>(blk + kv_codes_offset(D, 1, v0 + 8) + g * (4 * VW), r2);
+        lds_words<4 * VW>(blk + kv_codes_offset(D, 1, v1 + 8) + g * (4 * VW), r3);
 #pragma unroll
-        for (int w = 0; w < VW; ++w)
+        for (int i = 0; i < VW; ++i)
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
-            uint32_t xa = prmt(r0[w], r1[w], hf ? 0x7632 : 0x5410), xb = prmt(r2[w], r3[w], hf ? 0x7632 : 0x5410);
+            // row g: the even channel's code; row g + 8: the whole byte, even + 16 odd (an exact fp16 too), which takes no
+            // second mask: the odd channel's sum is the difference, once at the end
+            uint32_t xa = prmt(r0[i], r1[i], hf ? 0x7632 : 0x5410), xb = prmt(r2[i], r3[i], hf ? 0x7632 : 0x5410);
 #pragma unroll
             for (int by = 0; by < 2; ++by) {
+              const uint32_t ya = by ? prmt(xa, 0u, 0x4341) : xa & 0x00FF00FFu, yb = by ? prmt(xb, 0u, 0x4341) : xb & 0x00FF00FFu;
 #pragma unroll
-              for (int n = 0; n < NQ; ++n)
-                mma_16816(oacc[n][w * 4 + hf * 2 + by], xa & 0x000F000Fu, xa & 0x00F000F0u, xb & 0x000F000Fu, xb & 0x00F000F0u, pb[n][0], pb[n][1]);
-              xa >>= 8;
-              xb >>= 8;
+              for (int n = 0; n < NQ; ++n) {
+                float* o = oacc[n][i * 4 + hf * 2 + by];
+                mma_codes(oacc[n][i * 4 + hf * 2 + by], ya & 0x000F000Fu, ya, yb & 0x000F000Fu, yb, pb[n][0], pb[n][1], o[0], o[1], o[2], o[3]);
+              }
             }
           }
       }
-      __syncwarp();  // every lane has read the slot
-      if (((j + kAttnStages) & 31) == 0) {
-        // the block to be issued next is the first of a new set of 32 page numbers
-        const int k = (j + kAttnStages) >> 5;
-        if (k & 1) pages_now = fetch_pages(k + 1);
-        else pages_next = fetch_pages(k + 1);
+    };
+
+    int row0 = (seg.first * kAttnWarps + warp) * kSlotRows;
+    for (int j = 0; j < n_slots; ++j, row0 += kUnitRows) {
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar + 8 * slot, (phase >> slot) & 1u, kAttnWaitNs))) {
+        dead = true;
+        if (lane == 0 && p.status != nullptr) atomicExch(p.status, kStatusAttnTimeout);
+        break;
       }
-      issue(j + kAttnStages);
+      phase ^= 1u << slot;
+      const uint8_t* base = ring + slot * kSlot;
+      const uint32_t absent = (gone >> (kSlotBlocks * slot)) & kSlotMask;
+      if (row0 + kSlotRows - 1 <= min_limit && absent == 0) {
+#pragma unroll
+        for (int h = 0; h < kSlotBlocks / 2; ++h) consume(base + h * (2 * SB), 0, 0u, std::false_type{});
+      } else {
+#pragma unroll 1
+        for (int h = 0; h < kSlotBlocks / 2; ++h)
+          if (row0 + h * kPairRows < sq.len) consume(base + h * (2 * SB), row0 + h * kPairRows, (absent >> (2 * h)) & 3u, std::true_type{});
+      }
+      __syncwarp();  // every lane has read the slot
+      if (j + 1 < n_slots) copy_next();  // (the last one's is parked in first)
+      slot = slot + 1 == S ? 0 : slot + 1;
     }
 
-    // ---- the four warps' sums meet in shared memory (each parks its own in its ring, which is empty now) ----
-    float* park = reinterpret_cast<float*>(my_smem);
-    __syncwarp();
+    // ---- the next segment: its first rows are on their way already, its queries are asked for now ----
+    const uint32_t u_next = u + seg.len;
+    const Segment here = seg;
+    if (u_next < ue) {
+      settle(w, u_next);
+      seg = segment_at(w, u_next);
+      load_queries(w.sq, seg);
+    }
+
+    // ---- the four warps' sums meet in shared memory ----
+    float* park = reinterpret_cast<float*>(ring + (slot == 0 ? S - 1 : slot - 1) * kSlot);
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -459,55 +596,43 @@ __global__ void __launch_bounds__(kAttnThreads, NQ == 1 ? 4 : 3) fg_kv_attention
           z += __shfl_xor_sync(0xffffffffu, z, off);
         }
         const int col = n * 8 + 2 * c + q;
+        if (n_slots > 0) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          // accumulator row g holds the even channel (low nibble), row g + 8 the odd one
-          const float2 v = make_float2(fmaf(oacc[n][t][q], 16777216.f, z), fmaf(oacc[n][t][2 + q], 1048576.f, z));
-          *reinterpret_cast<float2*>(park + col * D + g * (8 * VW) + 2 * t) = v;
+          for (int t = 0; t < MT; ++t) {
+            // accumulator row g holds the even channel (low nibble), row g + 8 even + 16 odd
+            const float2 v = make_float2(fmaf(oacc[n][t][q], 16777216.f, z), fmaf(oacc[n][t][2 + q] - oacc[n][t][q], 1048576.f, z));
+            *reinterpret_cast<float2*>(park + col * D + g * (8 * VW) + 2 * t) = v;
+          }
         }
         if (g == 0) {
-          park[COLS * D + col] = mref[n][q];
-          park[COLS * D + COLS + col] = dead ? NAN : l;
+          warp_max[warp][col] = n_slots == 0 || l == 0.f ? kNoMax : mref[n][q];
+          warp_norm[warp][col] = dead ? NAN : l;
         }
       }
+    if (lane == 0) warp_sums[warp] = n_slots > 0 ? park : nullptr;
     __syncthreads();
-    const bool whole = seg_len == sq.units;
-    float* part = p.partials + (cta * 2 + (u == ub ? 0 : 1)) * partial_floats(D, COLS);
-    // thread: four channels of every (kAttnThreads / (D / 4))th column
-    constexpr int TPC = D / 4;
-    const int d4 = (tid % TPC) * 4;
-    auto write_out = [&](int col, float4 v, float l) {
-      if (col >= cols) return;
-      const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
-      const int flat = tile * COLS + col;
-      const __half2 h0 = __floats2half2_rn(v.x * inv, v.y * inv), h1 = __floats2half2_rn(v.z * inv, v.w * inv);
-      *reinterpret_cast<uint2*>(p.out + static_cast<long long>(sq.q0 + flat / p.group) * p.ldo +
-                                static_cast<long long>(head * p.group + flat % p.group) * D + d4) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
-    };
+    const bool whole = here.len == static_cast<int>(sq.units);
+    float* part = p.partials + static_cast<size_t>(cta * 2 + (u == ub ? 0 : 1)) * partial_floats(D, COLS);
 #pragma unroll 1
-    for (int col = tid / TPC; col < COLS; col += kAttnThreads / TPC) {
-      float m = -INFINITY, l = 0.f;
+    for (int col = tid / TPC; col < cols; col += kAttnThreads / TPC) {
+      float m = kNoMax, l = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      float mw[kAttnWarps];
 #pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) {
-        mw[w] = reinterpret_cast<const float*>(smem + w * kWarpBytes)[COLS * D + col];
-        m = fmaxf(m, mw[w]);
-      }
+      for (int i = 0; i < kAttnWarps; ++i) m = fmaxf(m, warp_max[i][col]);
 #pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) {
-        const float* src = reinterpret_cast<const float*>(smem + w * kWarpBytes);
-        const float f = m == -INFINITY ? 1.f : ex2(mw[w] - m);
-        const float4 a = *reinterpret_cast<const float4*>(src + col * D + d4);
-        l = fmaf(f, src[COLS * D + COLS + col], l);
-        v.x = fmaf(f, a.x, v.x);
-        v.y = fmaf(f, a.y, v.y);
-        v.z = fmaf(f, a.z, v.z);
-        v.w = fmaf(f, a.w, v.w);
+      for (int i = 0; i < kAttnWarps; ++i) {
+        const float f = ex2(warp_max[i][col] - m);
+        l = fmaf(f, warp_norm[i][col], l);
+        if (warp_sums[i] != nullptr) {
+          const float4 a = *reinterpret_cast<const float4*>(warp_sums[i] + col * D + d4);
+          v.x = fmaf(f, a.x, v.x);
+          v.y = fmaf(f, a.y, v.y);
+          v.z = fmaf(f, a.z, v.z);
+          v.w = fmaf(f, a.w, v.w);
+        }
       }
       if (whole) {
-        write_out(col, v, l);
+        write_out(tile * COLS + col, head, sq.q0, v, l);
       } else {
         __stcg(reinterpret_cast<float4*>(part + col * D + d4), v);
         if (d4 == 0) {
@@ -516,61 +641,95 @@ __global__ void __launch_bounds__(kAttnThreads, NQ == 1 ? 4 : 3) fg_kv_attention
         }
       }
     }
+    fence_proxy_async();  // the parked sums have been read before copies overwrite them
+    __syncthreads();
+    if (n_slots > 0 && !dead) copy_next();
     if (!whole) {
-      // ---- an item of several CTAs: the last of them to get here joins the partials in CTA order ----
-      const long long last_u = item_u0 + sq.units - 1;
-      auto cta_of = [&](long long unit) {  // the CTA whose share holds `unit`
-        long long x = unit * G / total;
-        while (x + 1 < G && (x + 1) * total / G <= unit) ++x;
-        while (x > 0 && x * total / G > unit) --x;
-        return x;
-      };
-      const long long c_first = cta_of(item_u0), c_last = cta_of(last_u);
-      __syncthreads();
+      // Publish the partial and go on; who was last is looked at when the share is done.
       if (tid == 0) {
-        __threadfence();
-        const unsigned int t = atomicAdd(p.tickets + c_first, 1u);
-        fence_acq_rel_gpu();
-        ticket = t;
+        Pending& q = pending[n_pending];
+        q.first = here.item_u0 / chunk;
+        q.parts = (here.item_u0 + sq.units - 1) / chunk - q.first + 1;
+        q.first_slot = q.first * chunk < here.item_u0 ? 1 : 0;  // only the first CTA can have begun its share in an earlier item
+        q.cols = cols;
+        q.tile = tile;
+        q.head = head;
+        q.q0 = sq.q0;
+        q.ticket = add_release(p.tickets + q.first, 1u);  // the other threads' stores too: the barrier has ordered them before
       }
-      __syncthreads();
-      if (ticket == static_cast<unsigned int>(c_last - c_first)) {
-        // only the first contributor can have begun its share in an earlier item
-        const int first_slot = c_first * total / G < item_u0 ? 1 : 0;
-        auto part_of = [&](long long x) {
-          const int slot = x == c_first ? first_slot : 0;
-          return p.partials + (x * 2 + slot) * partial_floats(D, COLS);
-        };
-#pragma unroll 1
-        for (int col = tid / TPC; col < cols; col += kAttnThreads / TPC) {
-          float m = -INFINITY, l = 0.f;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (long long x = c_first; x <= c_last; ++x) m = fmaxf(m, __ldcg(part_of(x) + COLS * D + col));
-#pragma unroll 4
-          for (long long x = c_first; x <= c_last; ++x) {
-            const float* src = part_of(x);
-            const float mx = __ldcg(src + COLS * D + col);
-            const float f = m == -INFINITY ? 1.f : ex2(mx - m);
-            const float4 a = __ldcg(reinterpret_cast<const float4*>(src + col * D + d4));
-            l = fmaf(f, __ldcg(src + COLS * D + COLS + col), l);
-            v.x = fmaf(f, a.x, v.x);
-            v.y = fmaf(f, a.y, v.y);
-            v.z = fmaf(f, a.z, v.z);
-            v.w = fmaf(f, a.w, v.w);
-          }
-          write_out(col, v, l);
-        }
-        if (tid == 0) p.tickets[c_first] = 0;  // ready for the next launch
-      }
+      ++n_pending;
     }
-    __syncthreads();          // the parked sums have been read
-    fence_proxy_async();      // ... and the copies of the next segment may overwrite them
-    u += seg_len;
+    u = u_next;
+  }
+
+  // ---- items of several CTAs: the last of them to get here joins the partials in CTA order ----
+  if (n_pending > 0) {
+    __syncthreads();
+    fence_acq_rel_gpu();
+  }
+  for (int k = 0; k < n_pending; ++k) {
+    const Pending q = pending[k];
+    if (q.ticket != q.parts - 1) continue;
+    const float* first = p.partials + static_cast<size_t>(q.first * 2) * partial_floats(D, COLS);
+    auto part_of = [&](uint32_t x) { return first + static_cast<size_t>(2 * x + (x == 0 ? q.first_slot : 0)) * partial_floats(D, COLS); };
+    // With L2 most of a microsecond away it is the number of dependent passes that counts: two columns of a thread and kJoin
+    // partials of each are asked for at once, the maxima among them.
+    constexpr int kStep = kAttnThreads / TPC;
+#pragma unroll 1
+    for (int col0 = tid / TPC; col0 < q.cols; col0 += 2 * kStep) {
+      float m[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
+      float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 1
+      for (uint32_t x0 = 0; x0 < q.parts; x0 += kJoin) {
+        float4 a[kJoin][2];
+        float mx[kJoin][2], lx[kJoin][2];
+#pragma unroll
+        for (uint32_t i = 0; i < kJoin; ++i)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            if (x0 + i < q.parts && col0 + y * kStep < q.cols) {
+              const float* src = part_of(x0 + i);
+              const int col = col0 + y * kStep;
+              a[i][y] = __ldcg(reinterpret_cast<const float4*>(src + col * D + d4));
+              mx[i][y] = __ldcg(src + COLS * D + col);
+              lx[i][y] = __ldcg(src + COLS * D + COLS + col);
+            } else {
+              a[i][y] = make_float4(0.f, 0.f, 0.f, 0.f);
+              mx[i][y] = kNoMax;
+              lx[i][y] = 0.f;
+            }
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float top = m[y];
+#pragma unroll
+          for (uint32_t i = 0; i < kJoin; ++i) top = fmaxf(top, mx[i][y]);
+          const float back = ex2(m[y] - top);
+          m[y] = top;
+          l[y] *= back;
+          v[y].x *= back;
+          v[y].y *= back;
+          v[y].z *= back;
+          v[y].w *= back;
+#pragma unroll
+          for (uint32_t i = 0; i < kJoin; ++i) {
+            const float f = ex2(mx[i][y] - top);
+            l[y] = fmaf(f, lx[i][y], l[y]);
+            v[y].x = fmaf(f, a[i][y].x, v[y].x);
+            v[y].y = fmaf(f, a[i][y].y, v[y].y);
+            v[y].z = fmaf(f, a[i][y].z, v[y].z);
+            v[y].w = fmaf(f, a[i][y].w, v[y].w);
+          }
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        if (col0 + y * kStep < q.cols) write_out(q.tile * COLS + col0 + y * kStep, q.head, q.q0, v[y], l[y]);
+    }
+    if (tid == 0) p.tickets[q.first] = 0;  // ready for the next launch
   }
   if (dead) {
     // a wait gave up: copies that are still in flight get time to land before the shared memory goes away
-    for (int s = 0; s < kAttnStages; ++s) mbar_wait_bounded(bar + 8 * s, (phase >> s) & 1u, kAttnWaitNs / 10);
+    for (int i = 0; i < S; ++i) mbar_wait_bounded(bar + 8 * i, (phase >> i) & 1u, kAttnWaitNs / 10);
   }
 }
 
@@ -598,7 +757,11 @@ extern "C" int fg_kv_attention_int4(const void* q, long long ldq, void* out, lon
   if (q_starts == nullptr && tokens != batch) return FG_ERR_SHAPE;
   if (tokens > 0x7fffffffLL / q_heads || static_cast<long long>(table_width) * page_size > 0x7fffffffLL - 2 * kUnitRows) return FG_ERR_SHAPE;
   if (ldq < static_cast<long long>(q_heads) * d || ldo < static_cast<long long>(q_heads) * d || (ldq % 8) != 0 || (ldo % 8) != 0) return FG_ERR_SHAPE;
-  if (!(scale > 0.f) || !(scale <= 3.0e38f)) return FG_ERR_SHAPE;
+  if (!(scale > 0.f) || !(scale <= kMaxScale)) return FG_ERR_SHAPE;
+  // work units and block numbers are 32-bit in the kernel; an upper bound of both, whatever the lengths turn out to be
+  const long long group = q_heads / kv_heads;
+  const double most_units = (static_cast<double>(tokens) * group / 8 + batch) * kv_heads * (static_cast<double>(table_width) * page_size / kUnitRows + 1);
+  if (most_units >= 2147483648.0 || static_cast<double>(num_pages) * kv_heads * (page_size / kKvBlock) >= 4294967295.0) return FG_ERR_SHAPE;
   if (!host::aligned(q, 16) || !host::aligned(out, 16) || !host::aligned(pages, 16) || !host::aligned(block_table, 4) ||
       !host::aligned(seq_lens, 4) || !host::aligned(q_starts, 4) || !host::aligned(status_dev, 4))
     return FG_ERR_ALIGN;
@@ -625,15 +788,15 @@ extern "C" int fg_kv_attention_int4(const void* q, long long ldq, void* out, lon
   p.tickets = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(ws) + kAttnTicketsOffset);
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kAttnPartialsOffset);
   p.status = status_dev;
-  // One column tile of eight where a sequence's queries of one key/value head fit it, else sixteen.
+  // Eight columns where a sequence's queries of one key/value head fit them, else sixteen.  (Thirty-two, for 64 channels, leave
+  // eight warps on an SM: 33.7 us against 23.1 on 24 x 3000 rows with up to 40 columns a sequence.)
   const long long per_seq = (tokens + batch - 1) / batch * p.group;
-  const bool wide = per_seq > 8;
-  void (*kern)(const AttnParams) = d == 128 ? (wide ? fg_kv_attention_kernel<128, 2> : fg_kv_attention_kernel<128, 1>)
-                                            : (wide ? fg_kv_attention_kernel<64, 2> : fg_kv_attention_kernel<64, 1>);
-  const int cols = wide ? 16 : 8;
-  const int ring = kAttnStages * kv_block_bytes(d), park = cols * (d + 4) * 4;
-  const int smem = kAttnWarps * (ring > park ? ring : park);
+  int cols = 8;
+  if (per_seq > cols) cols = kAttnMaxCols;
+  void (*kern)(const AttnParams) = d == 128 ? (cols == 16 ? fg_kv_attention_kernel<128, 2> : fg_kv_attention_kernel<128, 1>)
+                                   : (cols == 16 ? fg_kv_attention_kernel<64, 2> : fg_kv_attention_kernel<64, 1>);
+  const int smem = attn_smem_bytes(d, cols);
   if ((st = host::opt_in_smem(reinterpret_cast<const void*>(kern), smem)) != FG_OK) return st;
-  const int grid = min(kAttnMaxGrid, dev.sm_count * (wide ? 3 : 4));
+  const int grid = min(kAttnMaxGrid, dev.sm_count * attn_ctas_per_sm(cols));
   return host::launch(kern, dim3(grid), dim3(kAttnThreads), smem, reinterpret_cast<cudaStream_t>(stream), true, p);
 }

@@ -54,26 +54,41 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return q;
 }
 
+// Codes of four values as 16 bits: clamped, rounded to integers by adding and taking away 1.5 * 2^23 (to nearest, ties to
+// even), and put together as c0 + 16 c1 + 256 c2 + 4096 c3, which 32 bits hold exactly.
+// The quotient is the product with 1 / scale and one step of iterative refinement from its remainder: fp16 values often lie
+// exactly between two codes, where the bare product would pick either.
+__device__ __forceinline__ uint32_t codes4(const float* x, float low, float scale, float inv) {
+  float c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float y = x[i] - low;
+    float v = y * inv;
+    v = fmaf(fmaf(-v, scale, y), inv, v);
+    v = fminf(fmaxf(v, 0.f), 15.f);  // NaN: 0
+    c[i] = __fsub_rn(__fadd_rn(v, 12582912.f), 12582912.f);
+  }
+  return static_cast<uint32_t>(__float2int_rn(fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0])));
+}
+
 // D/16 lanes take a row: lane i the channels 8i.. of its lower half and the matching 8 of its upper half, so that both
-// kinds of rotation pair channels within one lane (i with i + D/2, or 2i with 2i + 1).  `HPT` consecutive heads of one
-// token go to the same lanes: their loads are in flight together and the angles are read once.
+// kinds of rotation pair channels within one lane (i with i + D/2, or 2i with 2i + 1).  blockIdx.y picks HPT consecutive
+// heads of the list queries, keys, values: whether a row is only turned or also quantised is the same for a whole CTA, and
+// one token's heads in a lane have their loads in flight together and share its angles.
 template <int D, int HPT>
 __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendParams p) {
   constexpr int LPR = D / 16;  // lanes per row
   const int lane = threadIdx.x % LPR;
-  const int heads = p.q_heads + 2 * p.kv.heads, groups = (heads + HPT - 1) / HPT;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kKvThreads / LPR) + threadIdx.x / LPR;
+  const int heads = p.q_heads + 2 * p.kv.heads, turned = p.q_heads + p.kv.heads;  // head numbers below `turned` are rotated
+  const long long token = static_cast<long long>(blockIdx.x) * (kKvThreads / LPR) + threadIdx.x / LPR;
+  const int head0 = blockIdx.y * HPT;
   griddep_launch_dependents();
   griddep_wait();
-  const long long token = unit / groups;
-  const int head0 = static_cast<int>(unit - token * groups) * HPT;
-  const bool active = token < p.tokens;
 
   // A padding token (negative slot) is left out whole; an index out of range too, and reported.
-  const long long slot = active ? p.slots[token] : -1;
-  bool go = slot >= 0;
+  const long long slot = token < p.tokens ? p.slots[token] : -1;
+  bool go = slot >= 0 && slot < p.kv.pages * p.kv.page_size;
   long long pos = 0;
-  if (go && slot >= p.kv.pages * p.kv.page_size) go = false;
   if (go && p.cos_sin != nullptr) {
     pos = p.positions[token];
     go = pos >= 0 && pos < p.positions_len;
@@ -87,15 +102,15 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
     raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
     if (go && h < heads) {
       const __half* src = h < p.q_heads ? p.q + token * p.ldq + static_cast<long long>(h) * D
-                          : h < p.q_heads + p.kv.heads
-                              ? p.k + token * p.ldk + static_cast<long long>(h - p.q_heads) * D
-                              : p.v + token * p.ldv + static_cast<long long>(h - p.q_heads - p.kv.heads) * D;
+                          : h < turned  ? p.k + token * p.ldk + static_cast<long long>(h - p.q_heads) * D
+                                        : p.v + token * p.ldv + static_cast<long long>(h - turned) * D;
       raw[i][0] = *reinterpret_cast<const uint4*>(src + 8 * lane);
       raw[i][1] = *reinterpret_cast<const uint4*>(src + D / 2 + 8 * lane);
     }
   }
+  const bool rotate = p.cos_sin != nullptr && head0 < turned;
   float cs[8], sn[8];
-  if (go && p.cos_sin != nullptr && head0 < p.q_heads + p.kv.heads) {
+  if (rotate && go) {
     const float* t = p.cos_sin + pos * D;
     // pairs (i, i + D/2): angles 8 lane..; pairs (2i, 2i + 1): angles 4 lane.. of the lower and of the upper half
     const int a0 = p.interleaved ? 4 * lane : 8 * lane, a1 = p.interleaved ? D / 4 + 4 * lane : 8 * lane + 4;
@@ -104,17 +119,22 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
     const float4 s1 = __ldg(reinterpret_cast<const float4*>(t + D / 2 + a1));
     cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w; cs[4] = c1.x; cs[5] = c1.y; cs[6] = c1.z; cs[7] = c1.w;
     sn[0] = s0.x; sn[1] = s0.y; sn[2] = s0.z; sn[3] = s0.w; sn[4] = s1.x; sn[5] = s1.y; sn[6] = s1.z; sn[7] = s1.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      cs[j] = 1.f;
+      sn[j] = 0.f;
+    }
   }
-  const long long page = go ? slot / p.kv.page_size : 0;
-  const int in_page = go ? static_cast<int>(slot - page * p.kv.page_size) : 0;
 
 #pragma unroll
   for (int i = 0; i < HPT; ++i) {
     const int h = head0 + i;
+    if (h >= heads) break;
     float lo[8], hi[8];
     unpack8(raw[i][0], lo);
     unpack8(raw[i][1], hi);
-    if (p.cos_sin != nullptr && h < p.q_heads + p.kv.heads && go) {
+    if (rotate && h < turned) {
       if (p.interleaved) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -139,6 +159,7 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
         *reinterpret_cast<uint4*>(dst + 8 * lane) = pack8(lo);
         *reinterpret_cast<uint4*>(dst + D / 2 + 8 * lane) = pack8(hi);
       }
+      continue;
     }
     // every lane of the warp takes part in the row reductions; rows that store nothing reduce zeros
     float mn = fminf(lo[0], hi[0]), mx = fmaxf(lo[0], hi[0]), bad = 0.f;
@@ -146,7 +167,7 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
     for (int j = 0; j < 8; ++j) {
       mn = fminf(mn, fminf(lo[j], hi[j]));
       mx = fmaxf(mx, fmaxf(lo[j], hi[j]));
-      bad += (lo[j] - lo[j]) + (hi[j] - hi[j]);  // 0, or NaN after an infinity or a NaN
+      bad = fmaf(lo[j], 0.f, fmaf(hi[j], 0.f, bad));  // 0, or NaN after an infinity or a NaN
     }
 #pragma unroll
     for (int off = LPR / 2; off >= 1; off >>= 1) {
@@ -154,28 +175,22 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
       bad += __shfl_xor_sync(0xffffffffu, bad, off);
     }
-    if (go && h >= p.q_heads && h < heads) {
-      const int which = h >= p.q_heads + p.kv.heads ? 1 : 0;
-      const int kv_head = h - p.q_heads - which * p.kv.heads;
+    if (go) {
+      const int which = h >= turned ? 1 : 0, kv_head = h - p.q_heads - which * p.kv.heads;
       const __half low_h = __float2half_rn(mn);
       const float low = __half2float(low_h);
       __half scale_h = __float2half_rn(__fdiv_rn(mx - low, 15.f));
       if (!(__half2float(scale_h) >= 5.9604644775390625e-8f)) scale_h = __ushort_as_half(1);
       if (bad != 0.f) scale_h = __ushort_as_half(0x7e00);  // the whole row reads back as NaN
-      const float scale = __half2float(scale_h);
-      uint32_t w[2] = {0, 0};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int a = min(15, max(0, __float2int_rn(__fdiv_rn(lo[j] - low, scale))));
-        const int b = min(15, max(0, __float2int_rn(__fdiv_rn(hi[j] - low, scale))));
-        w[0] |= static_cast<uint32_t>(a) << (4 * j);
-        w[1] |= static_cast<uint32_t>(b) << (4 * j);
-      }
-      const int row = in_page % kKvBlock;
+      const float scale = __half2float(scale_h), inv = __frcp_rn(scale);
+      const uint32_t w0 = codes4(lo, low, scale, inv) | (codes4(lo + 4, low, scale, inv) << 16);
+      const uint32_t w1 = codes4(hi, low, scale, inv) | (codes4(hi + 4, low, scale, inv) << 16);
+      const long long page = slot / p.kv.page_size;
+      const int in_page = static_cast<int>(slot - page * p.kv.page_size), row = in_page % kKvBlock;
       uint8_t* blk = kv_block_ptr(p.kv, D, page, kv_head, in_page / kKvBlock);
       uint8_t* codes = blk + kv_codes_offset(D, which, row);
-      *reinterpret_cast<uint32_t*>(codes + 4 * lane) = w[0];
-      *reinterpret_cast<uint32_t*>(codes + D / 4 + 4 * lane) = w[1];
+      *reinterpret_cast<uint32_t*>(codes + 4 * lane) = w0;
+      *reinterpret_cast<uint32_t*>(codes + D / 4 + 4 * lane) = w1;
       if (lane == 0) *reinterpret_cast<__half2*>(blk + kv_params_offset(D, which, row)) = __halves2half2(scale_h, low_h);
     }
   }
@@ -190,18 +205,17 @@ struct ReadParams {
 };
 
 // D/8 lanes take a row, eight channels each: a 4-byte load of codes becomes one 16-byte store, so that a warp's stores
-// cover whole 512-byte runs of the output, which is nine tenths of the traffic.  Two heads of keys and values a thread.
-template <int D>
+// cover whole rows of the output, which is nine tenths of the traffic.  blockIdx.y picks HPT consecutive heads; neighbouring
+// lane groups take neighbouring tokens, whose rows lie side by side in a block.
+template <int D, int HPT>
 __global__ void __launch_bounds__(kKvThreads) fg_kv_read_kernel(const ReadParams p) {
-  constexpr int LPR = D / 8, HPT = 2;
+  constexpr int LPR = D / 8;
   const int lane = threadIdx.x % LPR;
-  const int groups = (p.kv.heads + HPT - 1) / HPT;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kKvThreads / LPR) + threadIdx.x / LPR;
+  const long long token = static_cast<long long>(blockIdx.x) * (kKvThreads / LPR) + threadIdx.x / LPR;
+  const int head0 = blockIdx.y * HPT;
   griddep_launch_dependents();
   griddep_wait();
-  const long long token = unit / groups;
   if (token >= p.tokens) return;
-  const int head0 = static_cast<int>(unit - token * groups) * HPT;
   const long long slot = p.slots[token];
   if (slot < 0) return;
   if (slot >= p.kv.pages * p.kv.page_size) {
@@ -263,7 +277,7 @@ extern "C" int fg_kv_append_int4(const void* k, long long ldk, const void* v, lo
   if (k == nullptr || v == nullptr || slots == nullptr) return FG_ERR_NULL;
   if ((q == nullptr) != (q_out == nullptr) || (cos_sin == nullptr) != (positions == nullptr)) return FG_ERR_NULL;
   if (q != nullptr && cos_sin == nullptr) return FG_ERR_NULL;
-  if (tokens < 1 || (q != nullptr) != (q_heads > 0) || q_heads < 0 || q_heads > 65536 || kv_heads > 65536) return FG_ERR_SHAPE;
+  if (tokens < 1 || (q != nullptr) != (q_heads > 0) || q_heads < 0 || q_heads > 16384 || kv_heads > 16384) return FG_ERR_SHAPE;
   if (cos_sin != nullptr && positions_len < 1) return FG_ERR_SHAPE;
   if (ldk < static_cast<long long>(kv_heads) * d || ldv < static_cast<long long>(kv_heads) * d || (ldk % 8) != 0 || (ldv % 8) != 0)
     return FG_ERR_SHAPE;
@@ -295,12 +309,12 @@ extern "C" int fg_kv_append_int4(const void* k, long long ldk, const void* v, lo
   // Few rows: one a lane group, for latency; enough rows to fill the card twice over: four.
   const long long heads = q_heads + 2LL * kv_heads, rows_per_cta = kKvThreads / (d / 16);
   const bool many = tokens * heads >= 4 * 8 * rows_per_cta * dev.sm_count;
-  const int hpt = many ? 4 : 1;
-  const long long units = tokens * ((heads + hpt - 1) / hpt), grid = (units + rows_per_cta - 1) / rows_per_cta;
-  if (grid > 0x7fffffffLL) return FG_ERR_SHAPE;
+  const long long gx = (tokens + rows_per_cta - 1) / rows_per_cta, gy = (heads + (many ? 3 : 0)) / (many ? 4 : 1);
+  if (gx > 0x7fffffffLL || gy > 65535) return FG_ERR_SHAPE;
   void (*kern)(const AppendParams) = d == 128 ? (many ? fg_kv_append_kernel<128, 4> : fg_kv_append_kernel<128, 1>)
                                               : (many ? fg_kv_append_kernel<64, 4> : fg_kv_append_kernel<64, 1>);
-  return host::launch(kern, dim3(static_cast<unsigned>(grid)), dim3(kKvThreads), 0, reinterpret_cast<cudaStream_t>(stream), true, p);
+  return host::launch(kern, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), dim3(kKvThreads), 0,
+                      reinterpret_cast<cudaStream_t>(stream), true, p);
 }
 
 extern "C" int fg_kv_read_int4(const void* pages, long long num_pages, int page_size, int kv_heads, int d, const void* slots,
@@ -309,7 +323,7 @@ extern "C" int fg_kv_read_int4(const void* pages, long long num_pages, int page_
   int st = check_pages(pages, num_pages, kv_heads, page_size, d);
   if (st != FG_OK) return st;
   if (slots == nullptr || k_out == nullptr || v_out == nullptr) return FG_ERR_NULL;
-  if (tokens < 1 || kv_heads > 65536) return FG_ERR_SHAPE;
+  if (tokens < 1 || kv_heads > 16384) return FG_ERR_SHAPE;
   if (!host::aligned(k_out, 16) || !host::aligned(v_out, 16) || !host::aligned(slots, slots_64 ? 8 : 4) || !host::aligned(status_dev, 4))
     return FG_ERR_ALIGN;
   host::Device dev;
@@ -321,9 +335,12 @@ extern "C" int fg_kv_read_int4(const void* pages, long long num_pages, int page_
   p.v = static_cast<__half*>(v_out);
   p.status = status_dev;
   p.tokens = tokens;
-  const long long rows_per_cta = kKvThreads / (d / 8);
-  const long long units = tokens * ((kv_heads + 1) / 2), grid = (units + rows_per_cta - 1) / rows_per_cta;
-  if (grid > 0x7fffffffLL) return FG_ERR_SHAPE;
-  return host::launch(d == 128 ? fg_kv_read_kernel<128> : fg_kv_read_kernel<64>, dim3(static_cast<unsigned>(grid)), dim3(kKvThreads), 0,
+  const long long rows_per_cta = kKvThreads / (d / 8), gx = (tokens + rows_per_cta - 1) / rows_per_cta;
+  const bool many = tokens * kv_heads >= 4 * 8 * rows_per_cta * dev.sm_count;
+  const long long gy = (kv_heads + (many ? 3 : 0)) / (many ? 4 : 1);
+  if (gx > 0x7fffffffLL || gy > 65535) return FG_ERR_SHAPE;
+  void (*kern)(const ReadParams) = d == 128 ? (many ? fg_kv_read_kernel<128, 4> : fg_kv_read_kernel<128, 1>)
+                                            : (many ? fg_kv_read_kernel<64, 4> : fg_kv_read_kernel<64, 1>);
+  return host::launch(kern, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), dim3(kKvThreads), 0,
                       reinterpret_cast<cudaStream_t>(stream), true, p);
 }

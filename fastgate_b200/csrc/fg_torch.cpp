@@ -19,7 +19,6 @@
 #include <vector>
 
 #include "../../include/fastgate_b200.h"
-#include "fg_layout.h"
 #include "fg_torch.h"
 
 namespace {
@@ -410,20 +409,11 @@ void hgemm_tr(at::Tensor A, at::Tensor W, at::Tensor C) {
 
 }  // namespace
 
-StreamWorkspace stream_workspace(int64_t device, cudaStream_t stream, int64_t N) {
+StreamWorkspace linear_workspace(int64_t device, cudaStream_t stream, int64_t N) {
+  const size_t bytes = fg_workspace_bytes(static_cast<int>(std::max<int64_t>(N, 65536)));
+  if (void* p = graph_workspace(static_cast<int>(device), stream, kLinearWorkspace, bytes)) return {at::Tensor(), p, bytes};
   const Workspace w = workspace_for(static_cast<int>(device), stream, static_cast<int>(N));
-  return {w.buf, w.bytes};
-}
-
-StreamWorkspace captured_workspace(int64_t device, cudaStream_t stream, int64_t N) {
-  const size_t bytes = fg_workspace_bytes(static_cast<int>(N));
-  at::Tensor buf = at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
-  // only the header and the counters have to be clear; the partial tiles between them are written before they are read
-  char* p = static_cast<char*>(buf.data_ptr());
-  if (cudaMemsetAsync(p, 0, FG_WS_HEADER_BYTES, stream) != cudaSuccess ||
-      cudaMemsetAsync(p + FG_WS_TICKETS_OFFSET, 0, bytes - FG_WS_TICKETS_OFFSET, stream) != cudaSuccess)
-    throw std::runtime_error("fastgate_b200: CUDA call failed");
-  return {buf, bytes};
+  return {w.buf, w.buf.data_ptr(), w.bytes};
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

@@ -131,11 +131,6 @@ void add_rmsnorm(at::Tensor x, at::Tensor weight, at::Tensor out, OptTensor resi
 }
 
 // ---- linear on 8-bit activations -------------------------------------------------------------
-bool capturing(cudaStream_t stream) {
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  return cudaStreamIsCapturing(stream, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone;
-}
-
 void linear_int8(at::Tensor x8, at::Tensor W8, at::Tensor C, at::Tensor x_scales, OptTensor w_scales, OptTensor bias, OptTensor residual,
                  const std::string& act) {
   int code;
@@ -176,13 +171,13 @@ void linear_int8(at::Tensor x8, at::Tensor W8, at::Tensor C, at::Tensor x_scales
     bad_argument("the output may be the residual itself; otherwise it must not overlap the inputs");
   const c10::cuda::CUDAGuard guard(x8.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
-  const StreamWorkspace ws = capturing(stream) ? captured_workspace(device, stream, N) : stream_workspace(device, stream, N);
+  const StreamWorkspace ws = linear_workspace(device, stream, N);
   int st;
   {
     pybind11::gil_scoped_release nogil;
     st = fg_linear_w8a8(static_cast<const int8_t*>(x8.data_ptr()), static_cast<const int8_t*>(W8.data_ptr()), x_scales.data_ptr(), f32, ws_ptr,
                         C.data_ptr(), static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), bias_ptr, res_ptr, code,
-                        ws.buf.data_ptr(), ws.bytes, reinterpret_cast<fg_stream_t>(stream));
+                        ws.ptr, ws.bytes, reinterpret_cast<fg_stream_t>(stream));
   }
   check_status(st);
 }
@@ -240,7 +235,7 @@ void kv_append_int4(at::Tensor k, at::Tensor v, at::Tensor pages, at::Tensor slo
   int* sp = status_ptr(status, device);
   if (T == 0 || heads == 0) return;
   if (row_stride(k) % 8 || row_stride(v) % 8 || ldq % 8 || ldqo % 8) bad_argument("token strides must be multiples of 8 elements");
-  if (heads > 65536 || q_heads > 65536) bad_argument("too many heads");
+  if (heads > 16384 || q_heads > 16384) bad_argument("too many heads");
   const c10::cuda::CUDAGuard guard(k.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
   int st;
@@ -264,7 +259,7 @@ void kv_read_int4(at::Tensor pages, at::Tensor slots, at::Tensor k_out, at::Tens
   int* sp = status_ptr(status, device);
   if (overlap(k_out, v_out)) bad_argument("k_out and v_out must not overlap");
   if (T == 0 || heads == 0) return;
-  if (heads > 65536) bad_argument("too many heads");
+  if (heads > 16384) bad_argument("too many heads");
   const c10::cuda::CUDAGuard guard(k_out.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
   int st;
@@ -279,20 +274,18 @@ void kv_read_int4(at::Tensor pages, at::Tensor slots, at::Tensor k_out, at::Tens
 std::mutex g_attn_mu;
 std::map<std::pair<int64_t, int64_t>, at::Tensor> g_attn_ws;
 
-// One workspace per (device, stream), made on the first call.  A call that is being captured gets one of its own from the
-// graph's memory, cleared inside the graph: two graphs captured on one stream may be replayed side by side.
-at::Tensor attention_workspace(int64_t device, cudaStream_t stream) {
+// One workspace per (device, stream), made on the first call, or the graph's own while one is captured.
+StreamWorkspace attention_workspace(int64_t device, cudaStream_t stream) {
   const size_t bytes = fg_kv_attention_workspace_bytes();
-  auto make = [&] {
-    at::Tensor t = at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
-    check_status(fg_kv_attention_workspace_init(t.data_ptr(), bytes, reinterpret_cast<fg_stream_t>(stream)));
-    return t;
-  };
-  if (capturing(stream)) return make();
+  if (void* p = graph_workspace(static_cast<int>(device), stream, kAttentionWorkspace, bytes)) return {at::Tensor(), p, bytes};
   std::lock_guard<std::mutex> lk(g_attn_mu);
   at::Tensor& t = g_attn_ws[{device, reinterpret_cast<int64_t>(stream)}];
-  if (!t.defined()) t = make();
-  return t;
+  if (!t.defined()) {
+    at::Tensor made = at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+    check_status(fg_kv_attention_workspace_init(made.data_ptr(), bytes, reinterpret_cast<fg_stream_t>(stream)));
+    t = made;
+  }
+  return {t, t.data_ptr(), bytes};
 }
 
 void kv_attention_int4(at::Tensor q, at::Tensor pages, at::Tensor block_table, at::Tensor seq_lens, at::Tensor out, int64_t page_size,
@@ -323,7 +316,7 @@ void kv_attention_int4(at::Tensor q, at::Tensor pages, at::Tensor block_table, a
   }
   int* sp = status_ptr(status, device);
   const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(d));
-  if (!(sc > 0) || !(sc < 1e30)) bad_argument("scale must be positive");
+  if (!(sc > 0) || !(sc <= 1048576.0)) bad_argument("scale must be positive, and at most 2^20");
   if (T == 0 || B == 0) return;
   if (width < 1) bad_argument("block_table must have a column");
   const int64_t ldt = B > 1 ? block_table.stride(0) : width;
@@ -333,14 +326,14 @@ void kv_attention_int4(at::Tensor q, at::Tensor pages, at::Tensor block_table, a
   if (B > 0x7fffffff || width > 0x7fffffff || T > 0x7fffffff / q_heads) bad_argument("too many rows");
   const c10::cuda::CUDAGuard guard(q.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
-  const at::Tensor ws = attention_workspace(device, stream);
+  const StreamWorkspace ws = attention_workspace(device, stream);
   int st;
   {
     pybind11::gil_scoped_release nogil;
     st = fg_kv_attention_int4(q.data_ptr(), row_stride(q), out.data_ptr(), row_stride(out), T, static_cast<int>(q_heads),
                               static_cast<int>(heads), static_cast<int>(d), pages.data_ptr(), pages.size(0), static_cast<int>(page_size),
                               block_table.data_ptr<int>(), ldt, static_cast<int>(width), seq_lens.data_ptr<int>(), starts,
-                              static_cast<int>(B), static_cast<float>(sc), sp, ws.data_ptr(), static_cast<size_t>(ws.numel()),
+                              static_cast<int>(B), static_cast<float>(sc), sp, ws.ptr, ws.bytes,
                               reinterpret_cast<fg_stream_t>(stream));
   }
   check_status(st);

@@ -434,7 +434,7 @@ int fg_kv_read_int4(const void* pages, long long num_pages, int page_size, int k
  * among them, in the pages block_table[b * ldt + 0 ..] (table_width of them at most), and the query rows
  * q_starts[b] .. q_starts[b+1] - 1 (q_starts NULL: tokens == batch, row b).  Its i-th of n query rows is at position
  * seq_lens[b] - n + i and sees the rows up to there:
- *     out = sum_t softmax_t(scale * q . k_t) v_t
+ *     out = sum_t softmax_t(scale * q . k_t) v_t            0 < scale <= 2^20
  * A query that sees nothing (an empty sequence) gives zeros; rows of q outside every sequence leave out as it was; rows of
  * a page number out of range count as absent.  Scores, weights and sums in fp32, weights rounded to fp16 for the product
  * with the codes.  The split over the length depends on the lengths alone: results are reproducible bit by bit.
