@@ -244,6 +244,10 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
       if (dead) continue;
       tc_fence_after_sync();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + b * BN;
+      // The value of a sum before the activation, rounded step by step as in the other kernels on int8 activations.
+      auto value = [&](uint32_t sum, int col) {
+        return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(sum)), xs), col_scale[col]), col_bias[col]);
+      };
       // Thirty-two columns at a time; a row's pieces leave as 16-byte stores.
       auto emit = [&](int col, const float (&v)[32]) {  // col: column of the output
         if (!row) return;
@@ -260,8 +264,8 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
             float2 f = make_float2(v[8 * q + 2 * i], v[8 * q + 2 * i + 1]);
             if (res != nullptr) {
               const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&rw[i]));
-              f.x += a.x;
-              f.y += a.y;
+              f.x = __fadd_rn(f.x, a.x);
+              f.y = __fadd_rn(f.y, a.y);
             }
             const __half2 h = __floats2half2_rn(f.x, f.y);
             ow[i] = *reinterpret_cast<const uint32_t*>(&h);
@@ -281,9 +285,8 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
           float v[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float gv = fmaf(static_cast<float>(static_cast<int>(g[i])) * xs, col_scale[at + i], col_bias[at + i]);
-            const float uv = fmaf(static_cast<float>(static_cast<int>(u[i])) * xs, col_scale[at + 64 + i], col_bias[at + 64 + i]);
-            v[i] = act_fn<kActSilu>(gv) * uv;
+            const float gv = value(g[i], at + i), uv = value(u[i], at + 64 + i);
+            v[i] = __fmul_rn(act_fn<kActSilu>(gv), uv);
           }
           emit((n0 >> 1) + (c >> 1) * 64 + (c & 1) * 32, v);
         }
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
             float v[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              v[i] = act_fn<ACT>(fmaf(static_cast<float>(static_cast<int>(r[i])) * xs, col_scale[32 * c + i], col_bias[32 * c + i]));
+              v[i] = act_fn<ACT>(value(r[i], 32 * c + i));
             emit(n0 + 32 * c, v);
           }
         });

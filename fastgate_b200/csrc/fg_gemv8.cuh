@@ -1,0 +1,110 @@
+// int8 x int8 GEMV for one or two token rows (fg_linear_w8a8).
+//
+// A call of this size is a stream of the weight and the latencies around it: one warp takes R weight rows, its lanes stride
+// over k in 16-byte pieces, four dp4a per piece and token row, one integer reduction across the warp at the end.  No
+// ring, no partial tiles, no tickets: nothing stands between the last byte and the output.  The first pieces of the weight
+// are asked for before the previous kernel of the stream has finished (the weight depends on no kernel; the activations
+// are read after griddepcontrol.wait, through L1: every warp of an SM reads the same ones).
+// Measured on B200 (us, one / two rows; in brackets the streaming tcgen05 kernel, whose fixed costs are six microseconds):
+// 1024 x 1024 1.8 / 2.1 (6.1), 4096 x 4096 4.7 / 5.1 (8.1), 11008 x 4096 9.4 / 10.0 (11.9), 8192 x 8192 12.7 / 13.7 (14.8),
+// 28672 x 8192 36.8 / 38.9 (39.0; the weight at the measured copy bandwidth: 35.9).  Four rows take 4.5 to 52: L1 cannot
+// deliver the activations that often.
+// Weights above 60 MB: two rows of the weight per warp halve the reads of x (8192 x 8192 14.8 / 16.9 with one, 28672 x 8192
+// 36.8 / 39.1); below, one row per warp spreads the few rows wider (4096 x 4096 4.6 / 5.8 with two).
+#pragma once
+#include "fg_kernels.cuh"
+
+namespace fg {
+
+constexpr int kGemv8Warps = 4;
+constexpr int kGemv8MaxM = 2;
+constexpr int kGemv8Pieces = 4;                          // 16-byte pieces of each of its rows that a lane has in flight
+constexpr long long kGemv8TwoRowBytes = 60LL * 1000 * 1000;  // larger weights: two rows per warp
+
+struct Gemv8Params {
+  const int8_t* x;           // [M, K]
+  const int8_t* W;           // [N, K]
+  KParams out;               // C, scales, x_scales, bias, residual, act, M, N, K
+};
+
+template <int M, int R>
+__global__ void __launch_bounds__(kGemv8Warps * 32) fg_gemv8_kernel(const Gemv8Params p) {
+  const int lane = threadIdx.x & 31;
+  const long long wid = static_cast<long long>(blockIdx.x) * kGemv8Warps + (threadIdx.x >> 5);
+  const int K = p.out.K, N = p.out.N;
+  const bool gated = p.out.act == kActSiluGate;
+  // Rows of this warp: n0, n0 + step, ...: neighbours, or with the SiLU gate R/2 gate rows and the matching up rows 64 further.
+  const int first = static_cast<int>(wid * R);
+  int n[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = first / 2 + r / 2;  // gated: output column
+    n[r] = gated && R > 1 ? (j / 64) * 128 + (r & 1) * 64 + j % 64 : first + r;
+  }
+  griddep_launch_dependents();
+  if (first >= N) return;
+  const int pieces = K / 16;
+  const uint4* w[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) w[r] = reinterpret_cast<const uint4*>(p.W + static_cast<size_t>(n[r]) * K);
+  const uint4* x = reinterpret_cast<const uint4*>(p.x);
+  int acc[R][M];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[r][m] = 0;
+
+  uint4 q[kGemv8Pieces][R];
+  auto load = [&](int at) {
+#pragma unroll
+    for (int i = 0; i < kGemv8Pieces; ++i)
+#pragma unroll
+      for (int r = 0; r < R; ++r) q[i][r] = at + 32 * i < pieces ? __ldcs(w[r] + at + 32 * i) : make_uint4(0, 0, 0, 0);
+  };
+  load(lane);
+  griddep_wait();
+  for (int at = lane; at < pieces;) {
+#pragma unroll
+    for (int i = 0; i < kGemv8Pieces; ++i) {
+      if (at + 32 * i < pieces) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const uint4 v = __ldg(x + static_cast<size_t>(m) * pieces + at + 32 * i);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            acc[r][m] = __dp4a(static_cast<int>(q[i][r].x), static_cast<int>(v.x), acc[r][m]);
+            acc[r][m] = __dp4a(static_cast<int>(q[i][r].y), static_cast<int>(v.y), acc[r][m]);
+            acc[r][m] = __dp4a(static_cast<int>(q[i][r].z), static_cast<int>(v.z), acc[r][m]);
+            acc[r][m] = __dp4a(static_cast<int>(q[i][r].w), static_cast<int>(v.w), acc[r][m]);
+          }
+        }
+      }
+    }
+    at += 32 * kGemv8Pieces;
+    if (at - lane < pieces) load(at);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[r][m] = __reduce_add_sync(0xffffffffu, acc[r][m]);
+  // lane r M + m finishes output (m, n[r]); the gated pair (rows 2 i, 2 i + 1) is finished by the gate row's lane
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      if (lane != r * M + m) continue;
+      const float v = __int_as_float(acc[r][m]);
+      if (gated) {
+        if (R > 1 && (r & 1) == 0) store_gate<kOpW8A8NK>(p.out, m, n[r] / 128, n[r] % 128, v, __int_as_float(acc[r + (R > 1)][m]));
+      } else {
+        with_act(p.out.act, [&](auto tag) {
+          constexpr int ACT = decltype(tag)::value;
+          float y = scaled_sum<kOpW8A8NK>(p.out, m, n[r], v);
+          y = epilogue1<ACT, kOpW8A8NK>(p.out, m, n[r], y);
+          p.out.C[static_cast<size_t>(m) * N + n[r]] = __float2half_rn(y);
+        });
+      }
+    }
+}
+
+}  // namespace fg

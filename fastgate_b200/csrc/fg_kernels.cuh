@@ -415,8 +415,10 @@ __device__ __forceinline__ float x_scale(const KParams& p, int m) {
 template <int OP>
 __device__ __forceinline__ float scaled_sum(const KParams& p, int m, int n, float v) {
   if constexpr (OP == kOpW8A8NK) {
-    v = static_cast<float>(__float_as_int(v)) * x_scale(p, m);
-    if (p.scales != nullptr) v *= __half2float(p.scales[n]);
+    // products and sums rounded one by one (here, below and in the other kernels on int8 activations): a row then has the
+    // same bits whichever kernel computes it
+    v = __fmul_rn(static_cast<float>(__float_as_int(v)), x_scale(p, m));
+    if (p.scales != nullptr) v = __fmul_rn(v, __half2float(p.scales[n]));
   } else if ((OP == kOpW8A16NK || (OP == kOpW4A16NK && p.scale_groups <= 1)) && p.scales != nullptr) {
     v *= __half2float(p.scales[n]);  // one scale per output channel, applied in fp32
   }
@@ -429,19 +431,19 @@ __device__ __forceinline__ void store_gate(const KParams& p, int m, int tile, in
   g = scaled_sum<OP>(p, m, tile * kTileN + j, g);
   u = scaled_sum<OP>(p, m, tile * kTileN + 64 + j, u);
   if (p.bias != nullptr) {
-    g += __half2float(p.bias[tile * kTileN + j]);
-    u += __half2float(p.bias[tile * kTileN + 64 + j]);
+    g = __fadd_rn(g, __half2float(p.bias[tile * kTileN + j]));
+    u = __fadd_rn(u, __half2float(p.bias[tile * kTileN + 64 + j]));
   }
   const int n_out = tile * 64 + j, width = p.N >> 1;
-  float v = act_fn<kActSilu>(g) * u;
+  float v = OP == kOpW8A8NK ? __fmul_rn(act_fn<kActSilu>(g), u) : act_fn<kActSilu>(g) * u;
   if (p.residual != nullptr) v += __half2float(p.residual[static_cast<size_t>(m) * width + n_out]);
   p.C[static_cast<size_t>(m) * width + n_out] = __float2half_rn(v);
 }
 
 // bias, activation and residual of one output element (fp32).
-template <int ACT>
+template <int ACT, int OP = -1>
 __device__ __forceinline__ float epilogue1(const KParams& p, int m, int n, float v) {
-  if (p.bias != nullptr) v += __half2float(p.bias[n]);
+  if (p.bias != nullptr) v = OP == kOpW8A8NK ? __fadd_rn(v, __half2float(p.bias[n])) : v + __half2float(p.bias[n]);
   v = act_fn<ACT>(v);
   if (p.residual != nullptr) v += __half2float(p.residual[static_cast<size_t>(m) * p.N + n]);
   return v;
@@ -459,8 +461,8 @@ __device__ __forceinline__ __half2 finish_out2(const KParams& p, int m, int n, f
     v.y *= sc.y;
   }
   if (ACT != kActNone || p.bias != nullptr || p.residual != nullptr) {
-    v.x = epilogue1<ACT>(p, m, n, v.x);
-    v.y = epilogue1<ACT>(p, m, n + 1, v.y);
+    v.x = epilogue1<ACT, OP>(p, m, n, v.x);
+    v.y = epilogue1<ACT, OP>(p, m, n + 1, v.y);
   }
   return __floats2half2_rn(v.x, v.y);
 }

@@ -1,6 +1,6 @@
 // fg_linear_w8a8: int8 activations x int8 weights with scales, bias, activation and residual.
 //
-// Up to 128 token rows the weight is the traffic and the streaming kernel of the fp16 linears runs on it
+// One or two token rows: a GEMV (fg_gemv8_kernel).  Up to 128 the weight is still the traffic and the streaming kernel of the fp16 linears runs on it
 // (fg_umma_kernel<kOpW8A8NK>: the same bytes per stage, half the bytes per weight); above, the tensor cores are the
 // bound (fg_gemm8_kernel).
 #include <cuda.h>
@@ -8,6 +8,7 @@
 
 #include "../../include/fastgate_b200.h"
 #include "fg_gemm8.cuh"
+#include "fg_gemv8.cuh"
 #include "fg_host.h"
 #include "fg_layout.h"
 #include "fg_umma.cuh"
@@ -67,6 +68,28 @@ int run_streaming(const Args& a, const fg::host::Device& dev, void* ws, cudaStre
   p.act = a.act;
   p.ldc = a.N;
   return fg::host::launch(kern, dim3(pl.grid), dim3(fg::kUmmaThreads), pl.smem_bytes, stream, true, tmW, tmX, p);
+}
+
+int run_gemv(const Args& a, cudaStream_t stream) {
+  fg::Gemv8Params p = {};
+  p.x = static_cast<const int8_t*>(a.x);
+  p.W = static_cast<const int8_t*>(a.W);
+  p.out.C = static_cast<__half*>(a.C);
+  p.out.scales = static_cast<const __half*>(a.w_scales);
+  p.out.x_scales = a.x_scales;
+  p.out.x_scales_f32 = a.x_scales_f32;
+  p.out.bias = static_cast<const __half*>(a.bias);
+  p.out.residual = static_cast<const __half*>(a.residual);
+  p.out.act = a.act;
+  p.out.M = a.M;
+  p.out.N = a.N;
+  p.out.K = a.K;
+  // the SiLU gate pairs a gate row with its up row in one warp
+  const int R = a.act == FG_ACT_SILU_GATE || static_cast<long long>(a.N) * a.K > fg::kGemv8TwoRowBytes ? 2 : 1;
+  const long long warps = (a.N + R - 1) / R, grid = (warps + fg::kGemv8Warps - 1) / fg::kGemv8Warps;
+  void (*kern)(const fg::Gemv8Params) = a.M == 1 ? (R == 1 ? fg::fg_gemv8_kernel<1, 1> : fg::fg_gemv8_kernel<1, 2>)
+                                                 : (R == 1 ? fg::fg_gemv8_kernel<2, 1> : fg::fg_gemv8_kernel<2, 2>);
+  return fg::host::launch(kern, dim3(static_cast<unsigned>(grid)), dim3(fg::kGemv8Warps * 32), 0, stream, true, p);
 }
 
 template <int CG, int BN>
@@ -132,6 +155,7 @@ extern "C" int fg_linear_w8a8(const int8_t* x8, const int8_t* W8, const void* x_
   if (st != FG_OK) return st;
   const Args a = {x8, W8, x_scales, w_scales, x_scales_f32, C, M, N, K, bias, residual, act};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (M <= fg::kGemv8MaxM) return run_gemv(a, s);
   if (M <= kStreamRows) return run_streaming(a, dev, ws, s);
   // Pairs of CTAs once their tiles fill the card, single CTAs with smaller tiles below.
   const long long pair_tiles = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256);

@@ -116,7 +116,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 template <int OP, int ACT>
 __device__ __forceinline__ void store_out1(const KParams& p, int m, int n, float v) {
   v = scaled_sum<OP>(p, m, n, v);
-  if (ACT != kActNone || p.bias != nullptr || p.residual != nullptr) v = epilogue1<ACT>(p, m, n, v);
+  if (ACT != kActNone || p.bias != nullptr || p.residual != nullptr) v = epilogue1<ACT, OP>(p, m, n, v);
   const __half h = __float2half_rn(v);
   if (p.world == 0) {
     *out_ptr(p, m, n) = h;

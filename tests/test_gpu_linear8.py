@@ -43,7 +43,7 @@ def test_plain(M, N, K, dev):
 
 
 @pytest.mark.parametrize("act", ["none", "gelu", "gelu_tanh", "silu", "silu_gate"])
-@pytest.mark.parametrize("M", [1, 40, 100, 700])
+@pytest.mark.parametrize("M", [1, 2, 40, 100, 700])
 def test_epilogues(M, act, dev):
     N, K = 896, 512
     x, w, sx, sw, g = _data(M, N, K, M)
@@ -66,7 +66,7 @@ def test_scales_of_both_types_and_none(M, dev):
     _check(out, *ref.linear_int8(x, w, h, sw))
 
 
-@pytest.mark.parametrize("M", [1, 200, 600])
+@pytest.mark.parametrize("M", [1, 2, 5, 200, 600])
 def test_largest_sums(M, dev):
     """All -128 at the longest K allowed: the sum is 128 * 128 * 130944, just inside 32 bits."""
     K, N = 130944, 256
@@ -85,15 +85,20 @@ def test_largest_sums(M, dev):
 
 
 def test_rows_do_not_depend_on_their_company(dev):
-    """Exact sums: row i of every path (streaming with each tile height, single CTAs, pairs) has the same bits."""
-    x, w, sx, sw, _ = _data(2600, 8192, 384, 11)
+    """Exact sums and the same roundings after them: row i of every path (GEMV, streaming with each tile height, single CTAs,
+    pairs) has the same bits, whatever the epilogue."""
+    x, w, sx, sw, g = _data(2600, 8192, 384, 11)
     xd, wd, sxd, swd = x.to(dev), w.to(dev), sx.to(dev), sw.to(dev)
-    full = torch.empty(2600, 8192, dtype=torch.half, device=dev)
-    fg.linear_int8(xd, wd, full, sxd, swd)
-    for n in (1, 16, 31, 64, 128, 130, 513):
-        out = torch.empty(n, 8192, dtype=torch.half, device=dev)
-        fg.linear_int8(xd[:n], wd, out, sxd[:n], swd)
-        assert torch.equal(out, full[:n]), n
+    bias, res = torch.randn(8192, generator=g).half().to(dev), torch.randn(2600, 8192, generator=g).half().to(dev)
+    for act in ("none", "gelu_tanh", "silu_gate"):
+        width = 4096 if act == "silu_gate" else 8192
+        r = res[:, :width].contiguous()
+        full = torch.empty(2600, width, dtype=torch.half, device=dev)
+        fg.linear_int8(xd, wd, full, sxd, swd, bias, r, act)
+        for n in (1, 2, 16, 31, 64, 128, 130, 513):
+            out = torch.empty(n, width, dtype=torch.half, device=dev)
+            fg.linear_int8(xd[:n], wd, out, sxd[:n], swd, bias, r[:n], act)
+            assert torch.equal(out, full[:n]), (n, act)
 
 
 @pytest.mark.parametrize("M", [5, 300])
