@@ -132,8 +132,8 @@ def _load() -> ctypes.CDLL:
     L.fg_linear_host.argtypes = [i, vp, vp, vp, vp, vp, vp, i, i, i, vp, sz, vp]
     ll = ctypes.c_longlong
     L.fg_add_rmsnorm.argtypes = [vp, ll, vp, vp, vp, i, vp, i, vp, i, i, ctypes.c_float, vp]
-    L.fg_plan_w8a8.argtypes = [i, i, i, i, i, i, ctypes.POINTER(Plan)]  # internal: the streaming kernel of fg_linear_w8a8
-    L.fg_linear_w8a8.argtypes = [vp, vp, vp, i, vp, vp, i, i, i, vp, vp, i, vp, sz, vp]
+    L.fg_linear_w8a8_tiling.argtypes = [i, i, i, i, i, i]  # internal: the tiles of a call
+    L.fg_linear_w8a8.argtypes = [vp, vp, vp, i, vp, vp, i, i, i, vp, vp, i, vp, vp]
     L.fg_kv_append_int4.argtypes = [vp, ll, vp, ll, ll, i, i, vp, ll, i, vp, i, vp, ll, vp, i, vp, ll, vp, ll, i, i, vp, vp]
     L.fg_kv_read_int4.argtypes = [vp, ll, i, i, i, vp, i, ll, vp, vp, vp, vp]
     L.fg_kv_attention_workspace_bytes.argtypes = []

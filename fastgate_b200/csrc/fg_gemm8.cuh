@@ -1,43 +1,75 @@
-// int8 x int8 GEMM for many token rows (fg_linear_w8a8 above the streaming kernel's range).
+// int8 x int8 GEMM (fg_linear_w8a8 from three token rows on).
 //
 //   C[m, n] = act(sx[m] sw[n] sum_k x[m, k] W[n, k] + bias[n]) + residual[m, n]
 //
-// With hundreds of token rows the weight no longer bounds the call, the tensor cores do: 2 M N K operations against
-// M K + N K + 2 M N bytes.  tcgen05.mma.kind::i8, accumulators in tensor memory, 128-byte rows of k staged by TMA:
+// 2 M N K operations against M K + N K + 2 M N bytes: the weight's bytes bound the call up to a few hundred token rows, the
+// tensor cores above.  tcgen05.mma.kind::i8, accumulators in tensor memory, 128-byte rows of k staged by TMA:
 //
-//   CG = 2: two CTAs of a cluster share one 256 x BN tile (cta_group::2).  Each loads its own 128 token rows and half of
+//   CG = 2: two CTAs of a cluster share one 256 x 256 tile (cta_group::2).  Each loads its own 128 token rows and half of
 //           the tile's weight rows; the tensor cores of both read both halves of the weights.  A CTA alone at 128 x 256
 //           would fetch 48 KB from L2 per 128 k for the same 128 x 256 products, the pair fetches 32 KB per CTA, which is
 //           what L2 can deliver at full tensor rate.  One thread of the leading CTA issues every MMA.
-//   CG = 1: one CTA per 128 x BN tile, for problems with too few tiles to fill the card with pairs.
+//   CG = 1: one CTA per 128 x BN tile.  BN (32 to 256) is chosen so that the tiles of a small problem fill the card: the
+//           token rows beyond M cost no traffic and, next to the weight, no time.  Where even the narrowest tiles are too few,
+//           a cluster of 2 to 8 CTAs shares one, each with its part of k: the followers push their sums into the leader's
+//           shared memory, which has no copies in flight by then, and the leader finishes the tile.
 //
 // Persistent: CTAs (pairs) take tiles blockIdx.x, + gridDim.x, ... with the token tiles innermost, so that the tiles in
 // flight share weight rows in L2.  Two accumulators alternate: the epilogue of one tile overlaps the MMAs of the next.
-// Warps 0-3: epilogue (TMEM lane = token row), 4: copies, 5: MMA.  Sums are exact 32-bit integers.
+// The first ring-full of weights is asked for before the previous kernel of the stream has finished (the weight depends
+// on no kernel).  Warps 0-3: epilogue (TMEM lane = token row), 4: copies, 5: MMA.  Sums are exact 32-bit integers.
 #pragma once
 #include "fg_umma.cuh"
+#include "fg_w8a8.cuh"
 
 namespace fg {
 
 constexpr int kGemm8Threads = 192;
 
 struct Gemm8Params {
-  __half* C;
-  const void* x_scales;      // [M] fp32 or fp16
-  int x_scales_f32;
-  const __half* w_scales;    // [N] or nullptr
-  const __half* bias;        // [N] or nullptr
-  const __half* residual;    // [M, N] ([M, N/2] with the SiLU gate) or nullptr
-  int M, N, K;
-  int act;
+  W8A8Params out;
   int tiles_m, tiles_n;
   int stages;
-  int* status;
+  int splits;                // CG = 1: CTAs of a cluster that share a tile, each with its part of k (1: none)
+  int x_rows;                // token rows of one copy: 128, or fewer when M is below (the tile's other rows are left as they are:
+                             // their products are computed from whatever the slot holds and never stored)
 };
 
-__host__ __device__ constexpr int gemm8_stage_bytes(int cg, int bn) { return (128 + bn / cg) * 128; }
+__host__ __device__ constexpr int gemm8_block_bytes(int cg, int bn) { return (128 + bn / cg) * 128; }
+// Accumulation chains of a tile: consecutive MMAs into one accumulator wait for each other; tiles that leave tensor memory
+// free deal the k steps to two or four accumulators, which the epilogue adds up (exactly: integers).
+__host__ __device__ constexpr int gemm8_chains(int bn) { return bn <= 64 ? 4 : bn <= 128 ? 2 : 1; }
+__host__ __device__ constexpr uint32_t gemm8_tmem_cols(int bn) { return bn * gemm8_chains(bn) <= 128 ? 256 : 512; }
+// Weight rows of one copy: with the SiLU gate a tile narrower than a block of 128 takes gate rows and up rows separately.
+__host__ __device__ constexpr int gemm8_box_rows(int cg, int bn, bool gated) { return gated && bn / cg < 128 ? bn / 2 : bn / cg; }
+// k blocks of 128 that a stage holds: the barrier traffic around a stage costs its two threads as much as the copies and MMAs
+// of a block, so two where the ring stays three deep.
+__host__ __device__ constexpr int gemm8_blocks_per_stage(int cg, int bn) { return gemm8_block_bytes(cg, bn) <= 32768 ? 2 : 1; }
+__host__ __device__ constexpr int gemm8_stage_bytes(int cg, int bn) { return gemm8_blocks_per_stage(cg, bn) * gemm8_block_bytes(cg, bn); }
 __host__ __device__ constexpr int gemm8_smem_bytes(int cg, int bn, int stages) {
   return 1024 + stages * (gemm8_stage_bytes(cg, bn) + 16) + 64 + bn * 8;
+}
+
+// int8 x int8 -> int32: the same operand geometry in bytes as fp16, 32 k per instruction.
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor, kind::i8: signed A and B, 32-bit integer D, both K-major.
+__host__ __device__ constexpr uint32_t umma_idesc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((static_cast<uint32_t>(n) >> 3) << 17) | ((static_cast<uint32_t>(m) >> 4) << 24);
+}
+
+// One lane of a converged warp.  The loops of the copying and the MMA warp run on all lanes and only the instructions
+// themselves on one: what they take then stays in uniform registers, where those instructions want it.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 // ---- pairs of CTAs -----------------------------------------------------------------------
@@ -53,6 +85,9 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t smem_addr, uint32_t ran
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t mapped, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapped), "r"(v) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mapped_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapped_bar) : "memory");
@@ -90,12 +125,31 @@ __device__ __forceinline__ void gemm8_commit(uint32_t bar) {
   }
 }
 
+// kPiece columns of this thread's TMEM lane, the chains added up.
+template <int BN, int CHAINS, int PIECE>
+__device__ __forceinline__ void load_sums(uint32_t tbase, int col, uint32_t (&r)[PIECE]) {
+  uint32_t part[CHAINS][PIECE];
+#pragma unroll
+  for (int i = 0; i < CHAINS; ++i) {
+    if constexpr (PIECE == 32) tmem_ld32(tbase + i * BN + col, part[i]);
+    else tmem_ld16(tbase + i * BN + col, part[i]);
+  }
+  tmem_ld_wait();
+#pragma unroll
+  for (int j = 0; j < PIECE; ++j) {
+    r[j] = part[0][j];
+#pragma unroll
+    for (int i = 1; i < CHAINS; ++i) r[j] += part[i][j];
+  }
+}
+
 template <int CG, int BN>
 __global__ void __launch_bounds__(kGemm8Threads, 1)
     fg_gemm8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const Gemm8Params p) {
-  constexpr int kStage = gemm8_stage_bytes(CG, BN);
-  constexpr uint32_t kCols = 2 * BN;  // TMEM columns: two accumulators of BN
-  static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0, "tensor memory");
+  constexpr int kBlock = gemm8_block_bytes(CG, BN), kPer = gemm8_blocks_per_stage(CG, BN), kStage = kPer * kBlock;
+  constexpr uint32_t kCols = gemm8_tmem_cols(BN);  // two accumulators of BN columns
+  constexpr int kChains = gemm8_chains(BN);
+  static_assert(2 * kChains * BN <= static_cast<int>(kCols), "tensor memory");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -110,7 +164,11 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
   float* col_bias = col_scale + BN;                                                      // [BN]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const int splits = CG == 1 ? p.splits : 1;
+  const uint32_t in_cluster = CG == 2 || splits > 1 ? cluster_rank() : 0;
+  const uint32_t rank = CG == 2 ? in_cluster : 0;                         // which half of a pair's tile
+  const int part = CG == 1 ? static_cast<int>(in_cluster) : 0;           // which part of k
+  const int cluster = CG * splits;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(bar_full + 8 * s, 1);   // the leader's expect_tx for all CTAs' bytes
@@ -134,179 +192,245 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
   }
   tc_fence_before_sync();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();
+  if (cluster > 1) cluster_sync();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot_gen;
   griddep_launch_dependents();
-  griddep_wait();
+  const bool gated = p.out.act == kActSiluGate;
+  if (warp != 4) griddep_wait();
 
-  const int tiles = p.tiles_m * p.tiles_n, groups = gridDim.x / CG, group = blockIdx.x / CG;
-  const int k_blocks = p.K / 128;
+  const int tiles = p.tiles_m * p.tiles_n, groups = gridDim.x / cluster, group = blockIdx.x / cluster;
+  const int k_blocks = p.out.K / 128, all_stages = (k_blocks + kPer - 1) / kPer;
+  const int ks0 = part * all_stages / splits, ks1 = (part + 1) * all_stages / splits;  // this CTA's stages of every tile
   bool dead = false;
+  auto report = [&] {
+    if (p.out.status != nullptr) atomicExch(p.out.status, kStatusTimeout);
+  };
+
+  // Epilogue of a warp's 32 token rows of a tile (TMEM buffer b): scales, bias, activation, residual, kPiece columns at a time; a
+  // row's pieces leave as 16-byte stores.  more: followers' sums, [splits - 1][BN][128], or nullptr.
+  auto finish = [&](int n0, int m, bool row, float xs, uint32_t b, const uint32_t* more) {
+    const W8A8Params& q = p.out;
+    const int width = gated ? q.N >> 1 : q.N;
+    if (!__any_sync(0xffffffffu, row)) return;  // a small M: nothing to store for these rows
+    constexpr int kPiece = kChains <= 2 ? 32 : 16;
+    const uint32_t tbase = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + b * kChains * BN;
+    auto load_piece = [&](int col, uint32_t (&r)[kPiece]) {
+      load_sums<BN, kChains, kPiece>(tbase, col, r);
+      if (CG == 1 && more != nullptr)
+        for (int i = 0; i < splits - 1; ++i)
+#pragma unroll
+          for (int j = 0; j < kPiece; ++j) r[j] += more[(i * BN + col + j) * 128];
+    };
+    auto emit = [&](int col, const float (&v)[kPiece]) {  // col: column of the output
+      if (!row) return;
+      __half* dst = q.C + static_cast<size_t>(m) * width + col;
+      const __half* res = q.residual ? q.residual + static_cast<size_t>(m) * width + col : nullptr;
+#pragma unroll
+      for (int h = 0; h < kPiece / 8; ++h) {
+        uint4 r = make_uint4(0, 0, 0, 0), o;
+        if (res != nullptr) r = *reinterpret_cast<const uint4*>(res + 8 * h);
+        const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+        uint32_t* ow = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float2 f = make_float2(v[8 * h + 2 * i], v[8 * h + 2 * i + 1]);
+          if (res != nullptr) {
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&rw[i]));
+            f.x = __fadd_rn(f.x, a.x);
+            f.y = __fadd_rn(f.y, a.y);
+          }
+          const __half2 hv = __floats2half2_rn(f.x, f.y);
+          ow[i] = *reinterpret_cast<const uint32_t*>(&hv);
+        }
+        *reinterpret_cast<uint4*>(dst + 8 * h) = o;
+      }
+    };
+    auto value = [&](uint32_t sum, int col) { return w8a8_value(static_cast<int>(sum), xs, col_scale[col], col_bias[col]); };
+    if (gated) {
+      // kHalf gate columns, then the matching up columns, per block of 2 kHalf
+      constexpr int kHalf = BN < 128 ? BN / 2 : 64;
+#pragma unroll 1
+      for (int c = 0; c < BN / 2; c += kPiece) {  // column of the tile's output
+        const int at = c / kHalf * (2 * kHalf) + c % kHalf;
+        uint32_t g[kPiece], u[kPiece];
+        load_piece(at, g);
+        load_piece(at + kHalf, u);
+        if (n0 / 2 + c >= width) continue;
+        float v[kPiece];
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) v[i] = w8a8_gate(value(g[i], at + i), value(u[i], at + kHalf + i));
+        emit(n0 / 2 + c, v);
+      }
+    } else {
+      with_act(q.act, [&](auto tag) {
+        constexpr int ACT = decltype(tag)::value;
+#pragma unroll 1
+        for (int c = 0; c < BN; c += kPiece) {
+          uint32_t r[kPiece];
+          load_piece(c, r);
+          if (n0 + c >= q.N) continue;
+          float v[kPiece];
+#pragma unroll
+          for (int i = 0; i < kPiece; ++i) v[i] = w8a8_act<ACT>(value(r[i], c + i));
+          emit(n0 + c, v);
+        }
+      });
+    }
+  };
 
   if (warp == 4) {
-    if (lane == 0) {
-      tma_prefetch_desc(&tmX);
-      tma_prefetch_desc(&tmW);
-      const uint64_t policy = policy_evict_last();  // both operands are read again by other tiles
-      int s = 0, filled = 0;
-      uint32_t ph = 1;  // the slots start out empty
-      for (int t = group; t < tiles && !dead; t += groups) {
-        const int m0 = (t % p.tiles_m) * (128 * CG) + 128 * rank, n0 = (t / p.tiles_m) * BN + (BN / CG) * rank;
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait_bounded(bar_empty + 8 * s, ph, kWaitBudgetNs)) {
-            dead = true;
-            break;
-          }
-          const uint32_t dst = smem_base + s * kStage;
+    // ------------------------------------ copies ------------------------------------
+    const bool one = elect_one();
+    const uint64_t pol_x = policy_evict_last();                                              // read again by other tiles
+    const uint64_t pol_w = p.tiles_m > 1 ? policy_evict_last() : policy_evict_first();
+    const bool two_boxes = BN < 128 && gated;
+    const uint32_t full0 = CG == 2 ? map_to_rank(bar_full, 0) : bar_full;  // barriers of the leading CTA
+    int m_row = 0, n_row = 0;  // first token row and weight row of this CTA's copies
+    auto enter = [&](int t) {
+      const int tn = t / p.tiles_m, n0 = tn * BN;
+      m_row = (t - tn * p.tiles_m) * (128 * CG) + 128 * static_cast<int>(rank);
+      // with the gate and less than a block of 128: output columns n0 / 2 .., gate rows here, up rows 64 further on
+      n_row = two_boxes ? (n0 / 2 / 64) * 128 + n0 / 2 % 64 : n0 + (BN / CG) * static_cast<int>(rank);
+    };
+    auto load_x = [&](int slot, int ks) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int kb = ks * kPer + i;
+        if (kb < k_blocks) {
+          const uint32_t dst = smem_base + slot * kStage + i * kBlock;
+          if constexpr (CG == 1) tma_load_2d(dst, &tmX, full0 + 8 * slot, kb * 128, m_row, pol_x);
+          else tma_load_2d_pair(dst, &tmX, full0 + 8 * slot, kb * 128, m_row, pol_x);
+        }
+      }
+    };
+    auto load_w = [&](int slot, int ks) {
+      const int blocks = k_blocks - ks * kPer < kPer ? k_blocks - ks * kPer : kPer;
+      if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * slot, CG * blocks * (kBlock - (128 - p.x_rows) * 128));
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int kb = ks * kPer + i;
+        if (kb < k_blocks) {
+          const uint32_t dst = smem_base + slot * kStage + i * kBlock + 16384;
           if constexpr (CG == 1) {
-            mbar_arrive_expect_tx(bar_full + 8 * s, kStage);
-            tma_load_2d(dst, &tmX, bar_full + 8 * s, kb * 128, m0, policy);
-            tma_load_2d(dst + 16384, &tmW, bar_full + 8 * s, kb * 128, n0, policy);
+            tma_load_2d(dst, &tmW, full0 + 8 * slot, kb * 128, n_row, pol_w);
+            if (two_boxes) tma_load_2d(dst + BN / 2 * 128, &tmW, full0 + 8 * slot, kb * 128, n_row + 64, pol_w);
           } else {
-            const uint32_t lead = map_to_rank(bar_full + 8 * s, 0);
-            if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, 2 * kStage);
-            tma_load_2d_pair(dst, &tmX, lead, kb * 128, m0, policy);
-            tma_load_2d_pair(dst + 16384, &tmW, lead, kb * 128, n0, policy);
-          }
-          ++filled;
-          if (++s == S) {
-            s = 0;
-            ph ^= 1;
+            tma_load_2d_pair(dst, &tmW, full0 + 8 * slot, kb * 128, n_row, pol_w);
           }
         }
       }
-      // Every copy lands before the CTA may go: each filled slot has been consumed once more.  (After a wait that gave
-      // up the same waits, bounded too, are all that can be done.)
-      for (int i = 0; i < (filled < S ? filled : S); ++i) {
-        const int back = (s - 1 - i + 2 * S) % S;
-        const uint32_t use = static_cast<uint32_t>((filled - 1 - i) / S);
-        if (!mbar_wait_bounded(bar_empty + 8 * back, use & 1, kWaitBudgetNs)) dead = true;
-      }
-      if (dead) atomicExch(p.status, kStatusTimeout);
+    };
+    int s = 0, filled = 0;
+    uint32_t ph = 1;  // the slots start out empty
+    const int ahead = ks1 - ks0 < S ? ks1 - ks0 : S;  // of the first tile (there is one: no more groups than tiles)
+    enter(group);
+    if (one) {
+      tma_prefetch_desc(&tmX);
+      tma_prefetch_desc(&tmW);
+      for (int i = 0; i < ahead; ++i) load_w(i, ks0 + i);
     }
     __syncwarp();
+    griddep_wait();
+    for (int t = group; t < tiles && !dead; t += groups) {
+      if (t != group) enter(t);
+      for (int ks = ks0; ks < ks1; ++ks) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar_empty + 8 * s, ph, kWaitBudgetNs))) {
+          dead = true;
+          break;
+        }
+        if (one) {
+          if (filled >= ahead) load_w(s, ks);
+          load_x(s, ks);
+        }
+        __syncwarp();
+        ++filled;
+        if (++s == S) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    // Every copy lands before the CTA may go: each filled slot has been consumed once more.  (After a wait that gave
+    // up the same waits, bounded too, are all that can be done.)
+    for (int i = 0; i < (filled < S ? filled : S); ++i) {
+      const int back = (s - 1 - i + 2 * S) % S;
+      const uint32_t use = static_cast<uint32_t>((filled - 1 - i) / S);
+      if (!mbar_wait_bounded(bar_empty + 8 * back, use & 1, kWaitBudgetNs)) dead = true;
+    }
+    if (dead && lane == 0) report();
+    __syncwarp();
   } else if (warp == 5) {
-    if (lane == 0 && rank == 0) {
+    // ------------------------------------ MMA ------------------------------------
+    if (rank == 0) {
+      const bool one = elect_one();
       constexpr uint32_t idesc = umma_idesc_i8(128 * CG, BN);
       constexpr uint64_t desc = umma_smem_desc(0, 1, 64);
       int s = 0, n = 0;
       uint32_t ph = 0;
       for (int t = group; t < tiles && !dead; t += groups, ++n) {
         const uint32_t b = n & 1, use = n >> 1;
-        if (!mbar_wait_bounded(bar_acc_empty + 8 * b, (use & 1) ^ 1, kWaitBudgetNs)) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar_acc_empty + 8 * b, (use & 1) ^ 1, kWaitBudgetNs))) {
           dead = true;
           break;
         }
         tc_fence_after_sync();
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait_bounded(bar_full + 8 * s, ph, kWaitBudgetNs)) {
+        const uint32_t acc = tmem_base + b * kChains * BN;
+        for (int ks = ks0; ks < ks1; ++ks) {
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar_full + 8 * s, ph, kWaitBudgetNs))) {
             dead = true;
             break;
           }
-          tc_fence_after_sync();
-          const uint32_t at = smem_base + s * kStage;
-          const uint64_t a = desc | ((at >> 4) & 0x3FFFu), w = desc | (((at + 16384) >> 4) & 0x3FFFu);
+          if (one) {
+            const uint64_t at = desc | (((smem_base + s * kStage) >> 4) & 0x3FFFu);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) gemm8_mma<CG>(tmem_base + b * BN, a + 2 * k, w + 2 * k, idesc, (kb | k) != 0);
-          gemm8_commit<CG>(bar_empty + 8 * s);
+            for (int i = 0; i < kPer; ++i) {
+              if (i == 0 || ks * kPer + i < k_blocks) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  gemm8_mma<CG>(acc + k % kChains * BN, at + (i * kBlock / 16 + 2 * k), at + ((i * kBlock + 16384) / 16 + 2 * k), idesc,
+                                ks != ks0 || i != 0 || k >= kChains);
+              }
+            }
+            gemm8_commit<CG>(bar_empty + 8 * s);
+          }
+          __syncwarp();
           if (++s == S) {
             s = 0;
             ph ^= 1;
           }
         }
-        if (!dead) gemm8_commit<CG>(bar_acc_full + 8 * b);
+        if (!dead && one) gemm8_commit<CG>(bar_acc_full + 8 * b);
+        __syncwarp();
       }
-      if (dead) atomicExch(p.status, kStatusTimeout);
+      if (dead && lane == 0) report();
     }
     __syncwarp();
   } else {
-    const bool gated = p.act == kActSiluGate;
-    const int width = gated ? p.N >> 1 : p.N;
+    // ------------------------------------ epilogue ------------------------------------
+    const W8A8Params& q = p.out;
     int n = 0;
     for (int t = group; t < tiles; t += groups, ++n) {
       const int m = (t % p.tiles_m) * (128 * CG) + 128 * rank + 32 * warp + lane, n0 = (t / p.tiles_m) * BN;
       const uint32_t b = n & 1, use = n >> 1;
-      const bool row = m < p.M;
-      float xs = 0.f;
-      if (row) xs = p.x_scales_f32 ? static_cast<const float*>(p.x_scales)[m] : __half2float(static_cast<const __half*>(p.x_scales)[m]);
+      const bool row = m < q.M;
+      const float xs = row ? x_scale(q, m) : 0.f;
       named_bar_sync(1, 128);  // the previous tile's column values have been read
       for (int j = threadIdx.x; j < BN; j += 128) {
-        const bool in = n0 + j < p.N;
-        col_scale[j] = in && p.w_scales != nullptr ? __half2float(p.w_scales[n0 + j]) : 1.f;
-        col_bias[j] = in && p.bias != nullptr ? __half2float(p.bias[n0 + j]) : 0.f;
+        int w = n0 + j;  // weight row of column j
+        if (BN < 128 && gated) w = gate_row(n0 / 2 + j % (BN / 2)) + (j < BN / 2 ? 0 : 64);
+        col_scale[j] = w < q.N && q.w_scales != nullptr ? __half2float(q.w_scales[w]) : 1.f;
+        col_bias[j] = w < q.N && q.bias != nullptr ? __half2float(q.bias[w]) : 0.f;
       }
       named_bar_sync(1, 128);
       if (!dead && !__all_sync(0xffffffffu, mbar_wait_bounded(bar_acc_full + 8 * b, use & 1, 2 * kWaitBudgetNs))) {
         dead = true;
-        if (lane == 0) atomicExch(p.status, kStatusTimeout);
+        if (lane == 0) report();
       }
+      if (CG == 1 && splits > 1) break;  // the cluster's one tile: finished below, together
       if (dead) continue;
       tc_fence_after_sync();
-      const uint32_t tbase = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + b * BN;
-      // The value of a sum before the activation, rounded step by step as in the other kernels on int8 activations.
-      auto value = [&](uint32_t sum, int col) {
-        return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(sum)), xs), col_scale[col]), col_bias[col]);
-      };
-      // Thirty-two columns at a time; a row's pieces leave as 16-byte stores.
-      auto emit = [&](int col, const float (&v)[32]) {  // col: column of the output
-        if (!row) return;
-        __half* dst = p.C + static_cast<size_t>(m) * width + col;
-        const __half* res = p.residual ? p.residual + static_cast<size_t>(m) * width + col : nullptr;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint4 r = make_uint4(0, 0, 0, 0), o;
-          if (res != nullptr) r = *reinterpret_cast<const uint4*>(res + 8 * q);
-          const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
-          uint32_t* ow = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float2 f = make_float2(v[8 * q + 2 * i], v[8 * q + 2 * i + 1]);
-            if (res != nullptr) {
-              const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&rw[i]));
-              f.x = __fadd_rn(f.x, a.x);
-              f.y = __fadd_rn(f.y, a.y);
-            }
-            const __half2 h = __floats2half2_rn(f.x, f.y);
-            ow[i] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-          *reinterpret_cast<uint4*>(dst + 8 * q) = o;
-        }
-      };
-      if (gated) {
-#pragma unroll 1
-        for (int c = 0; c < BN / 64; ++c) {  // (128-row block, half): 32 gate columns and the matching up columns
-          const int at = (c >> 1) * 128 + (c & 1) * 32;
-          uint32_t g[32], u[32];
-          tmem_ld32(tbase + at, g);
-          tmem_ld32(tbase + at + 64, u);
-          tmem_ld_wait();
-          if (n0 + at >= p.N) continue;
-          float v[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float gv = value(g[i], at + i), uv = value(u[i], at + 64 + i);
-            v[i] = __fmul_rn(act_fn<kActSilu>(gv), uv);
-          }
-          emit((n0 >> 1) + (c >> 1) * 64 + (c & 1) * 32, v);
-        }
-      } else {
-        with_act(p.act, [&](auto tag) {
-          constexpr int ACT = decltype(tag)::value;
-#pragma unroll 1
-          for (int c = 0; c < BN / 32; ++c) {
-            uint32_t r[32];
-            tmem_ld32(tbase + 32 * c, r);
-            tmem_ld_wait();
-            if (n0 + 32 * c >= p.N) continue;
-            float v[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              v[i] = act_fn<ACT>(value(r[i], 32 * c + i));
-            emit(n0 + 32 * c, v);
-          }
-        });
-      }
+      finish(n0, m, row, xs, b, nullptr);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
@@ -316,10 +440,41 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
     }
   }
 
+  if constexpr (CG == 1) {
+    if (splits > 1) {
+      // Partial sums meet in the leader's ring: [follower][column][128 rows].  First barrier: the leader's MMAs have read
+      // everything that its copies brought.  Second: the followers' sums are there.
+      tc_fence_before_sync();
+      __syncwarp();
+      cluster_sync();
+      tc_fence_after_sync();
+      const uint32_t sums = smem_base;
+      if (warp < 4 && part > 0) {
+        const uint32_t to = map_to_rank(sums, 0) + (((part - 1) * BN) * 128 + 32 * warp + lane) * 4;
+        constexpr int kPiece = kChains <= 2 ? 32 : 16;
+#pragma unroll 1
+        for (int c = 0; c < BN; c += kPiece) {
+          uint32_t r[kPiece];
+          load_sums<BN, kChains, kPiece>(tmem_base + (static_cast<uint32_t>(warp * 32) << 16), c, r);
+#pragma unroll
+          for (int j = 0; j < kPiece; ++j) st_cluster(to + (c + j) * 512, r[j]);
+        }
+      }
+      __syncwarp();
+      cluster_sync();
+      if (warp < 4 && part == 0) {
+        const int m = (group % p.tiles_m) * 128 + 32 * warp + lane;
+        const bool row = m < p.out.M;
+        tc_fence_after_sync();
+        finish(group / p.tiles_m * BN, m, row && !dead, row ? x_scale(p.out, m) : 0.f, 0, reinterpret_cast<const uint32_t*>(smem_gen) + 32 * warp + lane);
+      }
+    }
+  }
+
   // ---- teardown: every MMA has completed (the epilogues have seen them) and the pair leaves together ----
   tc_fence_before_sync();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();
+  if (cluster > 1) cluster_sync();
   if (warp == 5) {
     tc_fence_after_sync();
     if constexpr (CG == 1) {
@@ -328,7 +483,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
       asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kCols) : "memory");
     }
   }
-  if constexpr (CG == 2) cluster_sync();
+  if (CG == 2) cluster_sync();
 }
 
 }  // namespace fg

@@ -5,14 +5,13 @@
 // ring, no partial tiles, no tickets: nothing stands between the last byte and the output.  The first pieces of the weight
 // are asked for before the previous kernel of the stream has finished (the weight depends on no kernel; the activations
 // are read after griddepcontrol.wait, through L1: every warp of an SM reads the same ones).
-// Measured on B200 (us, one / two rows; in brackets the streaming tcgen05 kernel, whose fixed costs are six microseconds):
-// 1024 x 1024 1.8 / 2.1 (6.1), 4096 x 4096 4.7 / 5.1 (8.1), 11008 x 4096 9.4 / 10.0 (11.9), 8192 x 8192 12.7 / 13.7 (14.8),
-// 28672 x 8192 36.8 / 38.9 (39.0; the weight at the measured copy bandwidth: 35.9).  Four rows take 4.5 to 52: L1 cannot
-// deliver the activations that often.
+// Measured on B200 (us, one / two rows): 1024 x 1024 1.8 / 2.1, 4096 x 4096 4.7 / 5.1, 11008 x 4096 9.4 / 10.0, 8192 x 8192
+// 12.7 / 13.7, 28672 x 8192 36.8 / 38.9 (the weight at the measured copy bandwidth: 35.9).  Four rows take 7 to 52, against
+// 8 to 38 in the tensor-core kernel: L1 cannot deliver the activations that often.
 // Weights above 60 MB: two rows of the weight per warp halve the reads of x (8192 x 8192 14.8 / 16.9 with one, 28672 x 8192
 // 36.8 / 39.1); below, one row per warp spreads the few rows wider (4096 x 4096 4.6 / 5.8 with two).
 #pragma once
-#include "fg_kernels.cuh"
+#include "fg_w8a8.cuh"
 
 namespace fg {
 
@@ -24,7 +23,7 @@ constexpr long long kGemv8TwoRowBytes = 60LL * 1000 * 1000;  // larger weights: 
 struct Gemv8Params {
   const int8_t* x;           // [M, K]
   const int8_t* W;           // [N, K]
-  KParams out;               // C, scales, x_scales, bias, residual, act, M, N, K
+  W8A8Params out;
 };
 
 template <int M, int R>
@@ -38,8 +37,7 @@ __global__ void __launch_bounds__(kGemv8Warps * 32) fg_gemv8_kernel(const Gemv8P
   int n[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int j = first / 2 + r / 2;  // gated: output column
-    n[r] = gated && R > 1 ? (j / 64) * 128 + (r & 1) * 64 + j % 64 : first + r;
+    n[r] = gated && R > 1 ? gate_row(first / 2 + r / 2) + (r & 1) * 64 : first + r;
   }
   griddep_launch_dependents();
   if (first >= N) return;
@@ -88,21 +86,24 @@ __global__ void __launch_bounds__(kGemv8Warps * 32) fg_gemv8_kernel(const Gemv8P
 #pragma unroll
     for (int m = 0; m < M; ++m) acc[r][m] = __reduce_add_sync(0xffffffffu, acc[r][m]);
   // lane r M + m finishes output (m, n[r]); the gated pair (rows 2 i, 2 i + 1) is finished by the gate row's lane
+  auto value = [&](int r, int m) {
+    return w8a8_value(acc[r][m], x_scale(p.out, m), p.out.w_scales ? __half2float(p.out.w_scales[n[r]]) : 1.f,
+                      p.out.bias ? __half2float(p.out.bias[n[r]]) : 0.f);
+  };
+  auto store = [&](int m, int width, int col, float y) {
+    const size_t at = static_cast<size_t>(m) * width + col;
+    if (p.out.residual != nullptr) y = __fadd_rn(y, __half2float(p.out.residual[at]));
+    p.out.C[at] = __float2half_rn(y);
+  };
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       if (lane != r * M + m) continue;
-      const float v = __int_as_float(acc[r][m]);
       if (gated) {
-        if (R > 1 && (r & 1) == 0) store_gate<kOpW8A8NK>(p.out, m, n[r] / 128, n[r] % 128, v, __int_as_float(acc[r + (R > 1)][m]));
+        if (R > 1 && (r & 1) == 0) store(m, N / 2, first / 2 + r / 2, w8a8_gate(value(r, m), value(r + (R > 1), m)));
       } else {
-        with_act(p.out.act, [&](auto tag) {
-          constexpr int ACT = decltype(tag)::value;
-          float y = scaled_sum<kOpW8A8NK>(p.out, m, n[r], v);
-          y = epilogue1<ACT, kOpW8A8NK>(p.out, m, n[r], y);
-          p.out.C[static_cast<size_t>(m) * N + n[r]] = __float2half_rn(y);
-        });
+        with_act(p.out.act, [&](auto tag) { store(m, N, n[r], w8a8_act<decltype(tag)::value>(value(r, m))); });
       }
     }
 }

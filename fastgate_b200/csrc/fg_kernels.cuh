@@ -45,7 +45,7 @@ constexpr int kMaxPeers = 8;          // ranks of one NVLink box
 constexpr int kTraceSlots = 16;       // 64-bit words per CTA of the built-in tracer
 constexpr unsigned long long kWaitBudgetNs = 2000000000ull;  // 2 s per wait, then give up
 
-enum { kOpF16KN = 0, kOpF16NK = 1, kOpW8A16NK = 2, kOpW4A16NK = 3, kOpW8A8NK = 4 };
+enum { kOpF16KN = 0, kOpF16NK = 1, kOpW8A16NK = 2, kOpW4A16NK = 3 };
 enum { kStatusOk = 0, kStatusTimeout = 6, kStatusBadLaunch = 7 };
 enum { kActNone = 0, kActGeluErf = 1, kActGeluTanh = 2, kActSilu = 3, kActSiluGate = 4 };
 
@@ -71,11 +71,6 @@ struct OpTraits<kOpW4A16NK> {
   static constexpr int chunkK = 256;      // 128 rows x 128 bytes of packed 4-bit weights
   static constexpr int xBoxes = 4;
 };
-template <>
-struct OpTraits<kOpW8A8NK> {              // int8 activations and weights: the byte geometry of kOpF16NK
-  static constexpr int chunkK = 128;
-  static constexpr int xBoxes = 1;
-};
 __host__ __device__ constexpr bool op_is_quantized(int op) { return op == kOpW8A16NK || op == kOpW4A16NK; }
 
 struct KParams {
@@ -83,8 +78,6 @@ struct KParams {
   const __half* scales;      // quantized ops: [N] per output channel, or [N, scale_groups] (int4), or nullptr
   int scale_groups;          // int4 op: scales per row; > 1: one per 128 k, applied inside the k loop
   uint32_t w4_magic;         // int4 op: half2(1024 + zero_point) twice
-  const void* x_scales;      // int8 activations: one scale per token row, fp32 or fp16
-  int x_scales_f32;
   float* partials;           // [grid][2][MT * 128]
   unsigned int* tickets;     // [tiles], zero between launches
   int* status;               // device status word
@@ -401,49 +394,22 @@ __device__ __forceinline__ __half* out_ptr(const KParams& p, int m, int n) {
   return p.C3 + static_cast<size_t>(m) * (p.N - p.split2) + (n - p.split2);
 }
 
-// Partial sums are fp32, or with int8 activations exact 32-bit integers carried in the bits of a float: such a sum
-// is the same whatever the split, and is turned into a real number once, with both scales.
-template <int OP>
-__device__ __forceinline__ void add_sum(float& a, float b) {
-  if constexpr (OP == kOpW8A8NK) a = __int_as_float(__float_as_int(a) + __float_as_int(b));
-  else a += b;
-}
-__device__ __forceinline__ float x_scale(const KParams& p, int m) {
-  return p.x_scales_f32 ? static_cast<const float*>(p.x_scales)[m] : __half2float(static_cast<const __half*>(p.x_scales)[m]);
-}
-// The value of a finished sum of row m, weight row n, before bias and activation.
-template <int OP>
-__device__ __forceinline__ float scaled_sum(const KParams& p, int m, int n, float v) {
-  if constexpr (OP == kOpW8A8NK) {
-    // products and sums rounded one by one (here, below and in the other kernels on int8 activations): a row then has the
-    // same bits whichever kernel computes it
-    v = __fmul_rn(static_cast<float>(__float_as_int(v)), x_scale(p, m));
-    if (p.scales != nullptr) v = __fmul_rn(v, __half2float(p.scales[n]));
-  } else if ((OP == kOpW8A16NK || (OP == kOpW4A16NK && p.scale_groups <= 1)) && p.scales != nullptr) {
-    v *= __half2float(p.scales[n]);  // one scale per output channel, applied in fp32
-  }
-  return v;
-}
-
-// One output of the SiLU-gated pair: g and u are the finished sums of gate row and up row `j` of tile `tile`.
-template <int OP>
+// One output of the SiLU-gated pair: g and u are the fp32 sums of gate row and up row `j` of tile `tile`.
 __device__ __forceinline__ void store_gate(const KParams& p, int m, int tile, int j, float g, float u) {
-  g = scaled_sum<OP>(p, m, tile * kTileN + j, g);
-  u = scaled_sum<OP>(p, m, tile * kTileN + 64 + j, u);
   if (p.bias != nullptr) {
-    g = __fadd_rn(g, __half2float(p.bias[tile * kTileN + j]));
-    u = __fadd_rn(u, __half2float(p.bias[tile * kTileN + 64 + j]));
+    g += __half2float(p.bias[tile * kTileN + j]);
+    u += __half2float(p.bias[tile * kTileN + 64 + j]);
   }
   const int n_out = tile * 64 + j, width = p.N >> 1;
-  float v = OP == kOpW8A8NK ? __fmul_rn(act_fn<kActSilu>(g), u) : act_fn<kActSilu>(g) * u;
+  float v = act_fn<kActSilu>(g) * u;
   if (p.residual != nullptr) v += __half2float(p.residual[static_cast<size_t>(m) * width + n_out]);
   p.C[static_cast<size_t>(m) * width + n_out] = __float2half_rn(v);
 }
 
 // bias, activation and residual of one output element (fp32).
-template <int ACT, int OP = -1>
+template <int ACT>
 __device__ __forceinline__ float epilogue1(const KParams& p, int m, int n, float v) {
-  if (p.bias != nullptr) v = OP == kOpW8A8NK ? __fadd_rn(v, __half2float(p.bias[n])) : v + __half2float(p.bias[n]);
+  if (p.bias != nullptr) v += __half2float(p.bias[n]);
   v = act_fn<ACT>(v);
   if (p.residual != nullptr) v += __half2float(p.residual[static_cast<size_t>(m) * p.N + n]);
   return v;
@@ -452,17 +418,14 @@ __device__ __forceinline__ float epilogue1(const KParams& p, int m, int n, float
 // Scale (int8 op), fused epilogue and rounding of two adjacent outputs of row m.
 template <int OP, int ACT>
 __device__ __forceinline__ __half2 finish_out2(const KParams& p, int m, int n, float2 v) {
-  if constexpr (OP == kOpW8A8NK) {
-    v.x = scaled_sum<OP>(p, m, n, v.x);
-    v.y = scaled_sum<OP>(p, m, n + 1, v.y);
-  } else if ((OP == kOpW8A16NK || (OP == kOpW4A16NK && p.scale_groups <= 1)) && p.scales != nullptr) {
+  if ((OP == kOpW8A16NK || (OP == kOpW4A16NK && p.scale_groups <= 1)) && p.scales != nullptr) {
     const float2 sc = __half22float2(*reinterpret_cast<const __half2*>(p.scales + n));
     v.x *= sc.x;
     v.y *= sc.y;
   }
   if (ACT != kActNone || p.bias != nullptr || p.residual != nullptr) {
-    v.x = epilogue1<ACT, OP>(p, m, n, v.x);
-    v.y = epilogue1<ACT, OP>(p, m, n + 1, v.y);
+    v.x = epilogue1<ACT>(p, m, n, v.x);
+    v.y = epilogue1<ACT>(p, m, n + 1, v.y);
   }
   return __floats2half2_rn(v.x, v.y);
 }
@@ -779,10 +742,10 @@ __device__ __forceinline__ void run_finisher(const KParams& p, const CtaRange& r
               for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                  add_sum<OP>(sum[i][h].x, v[j][i][h].x);
-                  add_sum<OP>(sum[i][h].y, v[j][i][h].y);
-                  add_sum<OP>(sum[i][h].z, v[j][i][h].z);
-                  add_sum<OP>(sum[i][h].w, v[j][i][h].w);
+                  sum[i][h].x += v[j][i][h].x;
+                  sum[i][h].y += v[j][i][h].y;
+                  sum[i][h].z += v[j][i][h].z;
+                  sum[i][h].w += v[j][i][h].w;
                 }
           }
           with_act(p.act, [&](auto tag) {
@@ -821,10 +784,10 @@ __device__ __forceinline__ void run_finisher(const KParams& p, const CtaRange& r
             for (int j = 0; j < 4; ++j)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                add_sum<OP>(sum[i].x, v[j][i].x);
-                add_sum<OP>(sum[i].y, v[j][i].y);
-                add_sum<OP>(sum[i].z, v[j][i].z);
-                add_sum<OP>(sum[i].w, v[j][i].w);
+                sum[i].x += v[j][i].x;
+                sum[i].y += v[j][i].y;
+                sum[i].z += v[j][i].z;
+                sum[i].w += v[j][i].w;
               }
           }
 #pragma unroll
@@ -833,10 +796,10 @@ __device__ __forceinline__ void run_finisher(const KParams& p, const CtaRange& r
             const float uz = __shfl_down_sync(0xffffffffu, sum[i].z, 16), uw = __shfl_down_sync(0xffffffffu, sum[i].w, 16);
             const int m = m0 + i;
             if (lane < 16 && m < p.M) {
-              store_gate<OP>(p, m, tile, 4 * lane, sum[i].x, ux);
-              store_gate<OP>(p, m, tile, 4 * lane + 1, sum[i].y, uy);
-              store_gate<OP>(p, m, tile, 4 * lane + 2, sum[i].z, uz);
-              store_gate<OP>(p, m, tile, 4 * lane + 3, sum[i].w, uw);
+              store_gate(p, m, tile, 4 * lane, sum[i].x, ux);
+              store_gate(p, m, tile, 4 * lane + 1, sum[i].y, uy);
+              store_gate(p, m, tile, 4 * lane + 2, sum[i].z, uz);
+              store_gate(p, m, tile, 4 * lane + 3, sum[i].w, uw);
             }
           }
         }

@@ -21,9 +21,8 @@
 #define FG_WS_PARTIALS_BYTES ((size_t)FG_MAX_GRID * 2 * FG_WS_PARTIAL_TILE_BYTES)
 #define FG_WS_TICKETS_OFFSET (FG_WS_HEADER_BYTES + FG_WS_PARTIALS_BYTES)
 
-/* op codes mirror FG_OP_* of the public header; int8 activations and weights (fg_linear_w8a8) have one of their own */
-#define FG_PLAN_OP_W8A8 4
-static inline int fg_chunk_k(int op) { return op == 3 ? 256 : op == 2 || op == FG_PLAN_OP_W8A8 ? 128 : 64; }
+/* op codes mirror FG_OP_* of the public header */
+static inline int fg_chunk_k(int op) { return op == 3 ? 256 : op == 2 ? 128 : 64; }
 /* activation boxes (64 k x m_tile rows, 128 B per row) that accompany one weight chunk */
 static inline int fg_x_boxes(int op) { return op == 3 ? 4 : op == 2 ? 2 : 1; }
 static inline int fg_chunk_bytes(int op, int m_tile) {
@@ -73,8 +72,6 @@ extern "C" int fg_plan_mma_sync(int op, int M, int N, int K, int sm_count, int s
                                 struct fg_plan_t* out); /* quantized ops: the mma.sync kernel's plan for any M */
 extern "C" int fg_plan_tiled(int op, int M, int N, int K, int sm_count, int smem_optin_bytes,
                              struct fg_plan_t* out);    /* never the row-split GEMV kernel */
-extern "C" int fg_plan_w8a8(int M, int N, int K, int sm_count, int smem_optin_bytes, int extra_smem_bytes,
-                            struct fg_plan_t* out);    /* the streaming kernel on int8 activations and weights */
 #endif
 #define FG_UMMA_Q_STAGING_BYTES 98304 /* three 32 KB buffers */
 static inline int fg_umma_q_smem_bytes(int op, int chunks, int stages);

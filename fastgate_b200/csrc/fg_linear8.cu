@@ -1,8 +1,6 @@
 // fg_linear_w8a8: int8 activations x int8 weights with scales, bias, activation and residual.
 //
-// One or two token rows: a GEMV (fg_gemv8_kernel).  Up to 128 the weight is still the traffic and the streaming kernel of the fp16 linears runs on it
-// (fg_umma_kernel<kOpW8A8NK>: the same bytes per stage, half the bytes per weight); above, the tensor cores are the
-// bound (fg_gemm8_kernel).
+// One or two token rows: a GEMV (fg_gemv8_kernel); more: a tensor-core kernel (fg_gemm8_kernel) with tiles chosen by size.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -11,118 +9,101 @@
 #include "fg_gemv8.cuh"
 #include "fg_host.h"
 #include "fg_layout.h"
-#include "fg_umma.cuh"
 
 namespace {
 
 using fg::host::aligned;
 
-constexpr int kStreamRows = 128;       // token rows the streaming kernel takes
 constexpr int kMaxK = 131072 - 128;    // k (-128)(-128) < 2^31
 
-struct Args {
-  const void *x, *W, *x_scales, *w_scales;
-  int x_scales_f32;
-  void* C;
-  int M, N, K;
-  const void *bias, *residual;
-  int act;
-};
-
-int run_streaming(const Args& a, const fg::host::Device& dev, void* ws, cudaStream_t stream) {
-  using StreamFn = void (*)(const CUtensorMap, const CUtensorMap, const fg::KParams);
-  const bool gate = a.act == FG_ACT_SILU_GATE;
-  fg_plan_t pl;
-  int st = fg_plan_w8a8(a.M, a.N, a.K, dev.sm_count, dev.smem_optin, gate ? static_cast<int>(fg::kGateXchBytes) : 0, &pl);
-  if (st != FG_OK) return st;
-  const StreamFn kern = pl.m_tile == 16   ? fg::fg_umma_kernel<fg::kOpW8A8NK, 16>
-                        : pl.m_tile == 32 ? fg::fg_umma_kernel<fg::kOpW8A8NK, 32>
-                        : pl.m_tile == 64 ? fg::fg_umma_kernel<fg::kOpW8A8NK, 64>
-                                          : fg::fg_umma_kernel<fg::kOpW8A8NK, 128>;
-  if ((st = fg::host::opt_in_smem(reinterpret_cast<const void*>(kern), pl.smem_bytes)) != FG_OK) return st;
-  CUtensorMap tmW, tmX;
-  if ((st = fg::host::encode_tensor(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.W, a.K, a.N, 128, 128)) != FG_OK) return st;
-  if ((st = fg::host::encode_tensor(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.x, a.K, a.M, 128, pl.m_tile)) != FG_OK) return st;
-  uint8_t* wsb = static_cast<uint8_t*>(ws);
-  fg::KParams p = {};
-  p.C = static_cast<__half*>(a.C);
-  p.scales = static_cast<const __half*>(a.w_scales);
-  p.scale_groups = 1;
-  p.x_scales = a.x_scales;
-  p.x_scales_f32 = a.x_scales_f32;
-  p.partials = reinterpret_cast<float*>(wsb + FG_WS_HEADER_BYTES);
-  p.tickets = reinterpret_cast<unsigned int*>(wsb + FG_WS_TICKETS_OFFSET);
-  p.status = reinterpret_cast<int*>(wsb);
-  p.M = a.M;
-  p.N = a.N;
-  p.K = a.K;
-  p.tiles = pl.tiles;
-  p.k_blocks = pl.k_blocks;
-  p.chunks_per_stage = pl.k_per_stage / fg_chunk_k(pl.op);
-  p.stages = pl.stages;
-  p.consumer_warps = pl.consumer_warps;
-  p.pdl = pl.pdl;
-  p.l2_prefetch = FG_L2_PREFETCH_BYTES / (p.chunks_per_stage * FG_CHUNK_W_BYTES);
-  p.bias = static_cast<const __half*>(a.bias);
-  p.residual = static_cast<const __half*>(a.residual);
-  p.act = a.act;
-  p.ldc = a.N;
-  return fg::host::launch(kern, dim3(pl.grid), dim3(fg::kUmmaThreads), pl.smem_bytes, stream, true, tmW, tmX, p);
-}
-
-int run_gemv(const Args& a, cudaStream_t stream) {
-  fg::Gemv8Params p = {};
-  p.x = static_cast<const int8_t*>(a.x);
-  p.W = static_cast<const int8_t*>(a.W);
-  p.out.C = static_cast<__half*>(a.C);
-  p.out.scales = static_cast<const __half*>(a.w_scales);
-  p.out.x_scales = a.x_scales;
-  p.out.x_scales_f32 = a.x_scales_f32;
-  p.out.bias = static_cast<const __half*>(a.bias);
-  p.out.residual = static_cast<const __half*>(a.residual);
-  p.out.act = a.act;
-  p.out.M = a.M;
-  p.out.N = a.N;
-  p.out.K = a.K;
+int run_gemv(const fg::W8A8Params& a, const int8_t* x, const int8_t* W, cudaStream_t stream) {
   // the SiLU gate pairs a gate row with its up row in one warp
   const int R = a.act == FG_ACT_SILU_GATE || static_cast<long long>(a.N) * a.K > fg::kGemv8TwoRowBytes ? 2 : 1;
   const long long warps = (a.N + R - 1) / R, grid = (warps + fg::kGemv8Warps - 1) / fg::kGemv8Warps;
   void (*kern)(const fg::Gemv8Params) = a.M == 1 ? (R == 1 ? fg::fg_gemv8_kernel<1, 1> : fg::fg_gemv8_kernel<1, 2>)
                                                  : (R == 1 ? fg::fg_gemv8_kernel<2, 1> : fg::fg_gemv8_kernel<2, 2>);
+  const fg::Gemv8Params p = {x, W, a};
   return fg::host::launch(kern, dim3(static_cast<unsigned>(grid)), dim3(fg::kGemv8Warps * 32), 0, stream, true, p);
 }
 
+// ---- tiles of the tensor-core kernel ------------------------------------------------------------
+struct Tiling {
+  int bn;      // weight rows of a tile
+  int cg;      // CTAs that share a tile's MMAs: 1 (128 token rows) or 2 (256)
+  int splits;  // CTAs that share a tile's k (cg 1)
+};
+
+struct TileCost {
+  int bn, cg;
+  double few_us, many_us;  // one block of 128 k on one CTA (pair), with one row of token tiles and with several
+};
+// Measured on B200 (M = 3 to 128 and 256 to 4096; N = 1024 to 28672, K = 4096 to 11008): time per wave less 3.5 us, over the
+// blocks of k.  Narrow tiles are bound by the issue of their four MMAs a block, wide ones by the tensor cores and L2.
+constexpr TileCost kTileCosts[] = {{32, 1, 0.148, 0.155}, {64, 1, 0.163, 0.18}, {96, 1, 0.175, 0.21}, {128, 1, 0.22, 0.25},
+                                   {192, 1, 0.265, 0.32}, {256, 1, 0.36, 0.40}, {256, 2, 0.36, 0.36}};
+constexpr double kSplitUs = 3.5;    // launch of clusters, two cluster barriers and the exchange between them
+constexpr double kDramBytesPerUs = 6.2e6;
+
+int stages_of(const TileCost& c, int smem_optin) {
+  const int s = (smem_optin - fg::gemm8_smem_bytes(c.cg, c.bn, 0)) / (fg::gemm8_stage_bytes(c.cg, c.bn) + 16);
+  return s < FG_MAX_STAGES ? s : FG_MAX_STAGES;
+}
+
+// The tiling with the least estimated time: per wave of tiles its blocks of k or its share of the bytes, whichever takes
+// longer (a last wave of a few tiles costs as much as a full one where the tensor cores bound it, little where memory does).
+Tiling choose_tiling(int M, int N, int K, bool gated, int sm_count, int smem_optin) {
+  const double dram = (static_cast<double>(N) * K + static_cast<double>(M) * K + 2.0 * M * N) / kDramBytesPerUs;
+  Tiling best = {128, 1, 1};
+  double best_us = 1e30;
+  for (const TileCost& c : kTileCosts) {
+    if (gated && (c.bn == 96 || c.bn == 192)) continue;  // a gate row and its up row belong to one tile
+    const long long tiles = static_cast<long long>((M + 128 * c.cg - 1) / (128 * c.cg)) * ((N + c.bn - 1) / c.bn);
+    const int per = fg::gemm8_blocks_per_stage(c.cg, c.bn), k_stages = (K / 128 + per - 1) / per;
+    const int ring = stages_of(c, smem_optin) * fg::gemm8_stage_bytes(c.cg, c.bn);
+    for (int s = 1; s <= (c.cg == 1 ? 8 : 1); s *= 2) {
+      // A cluster lives in one GPC: up to seven eighths of the SMs can be counted on.  Every CTA has a stage at least, and the
+      // followers' sums fit in the leader's ring.
+      if (s > 1 && (tiles * s > sm_count - sm_count / 8 || k_stages < s || (s - 1) * c.bn * 512 > ring)) break;
+      const long long at_once = s > 1 ? tiles : sm_count / c.cg;
+      const int blocks = s > 1 ? (k_stages + s - 1) / s * per : K / 128;
+      const double mma = blocks * (M <= 128 ? c.few_us : c.many_us);
+      const long long full = tiles / at_once, rest = tiles % at_once;
+      const double full_dram = dram * at_once / tiles, rest_dram = dram * rest / tiles;
+      const double us = full * (mma > full_dram ? mma : full_dram) + (rest ? (mma > rest_dram ? mma : rest_dram) : 0.0) + (s > 1 ? kSplitUs : 0.0);
+      if (us < best_us) {
+        best_us = us;
+        best = {c.bn, c.cg, s};
+      }
+    }
+  }
+  return best;
+}
+
 template <int CG, int BN>
-int run_gemm(const Args& a, const fg::host::Device& dev, void* ws, cudaStream_t stream) {
+int run_gemm(const fg::W8A8Params& a, const int8_t* x, const int8_t* W, int splits, const fg::host::Device& dev, cudaStream_t stream) {
   const auto kern = fg::fg_gemm8_kernel<CG, BN>;
-  int stages = (dev.smem_optin - fg::gemm8_smem_bytes(CG, BN, 0)) / (fg::gemm8_stage_bytes(CG, BN) + 16);
-  if (stages > FG_MAX_STAGES) stages = FG_MAX_STAGES;
+  const int stages = stages_of({BN, CG, 0.0, 0.0}, dev.smem_optin);
   if (stages < 2) return FG_ERR_PLAN;
   const int smem = fg::gemm8_smem_bytes(CG, BN, stages);
   int st = fg::host::opt_in_smem(reinterpret_cast<const void*>(kern), smem);
   if (st != FG_OK) return st;
+  const int x_rows = CG == 1 && a.M < 128 ? (a.M + 7) / 8 * 8 : 128;
+  const int w_rows = fg::gemm8_box_rows(CG, BN, a.act == FG_ACT_SILU_GATE);
   CUtensorMap tmW, tmX;
-  if ((st = fg::host::encode_tensor(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.x, a.K, a.M, 128, 128)) != FG_OK) return st;
-  if ((st = fg::host::encode_tensor(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.W, a.K, a.N, 128, BN / CG)) != FG_OK) return st;
+  if ((st = fg::host::encode_tensor(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, a.K, a.M, 128, x_rows)) != FG_OK) return st;
+  if ((st = fg::host::encode_tensor(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, W, a.K, a.N, 128, w_rows)) != FG_OK) return st;
   fg::Gemm8Params p = {};
-  p.C = static_cast<__half*>(a.C);
-  p.x_scales = a.x_scales;
-  p.x_scales_f32 = a.x_scales_f32;
-  p.w_scales = static_cast<const __half*>(a.w_scales);
-  p.bias = static_cast<const __half*>(a.bias);
-  p.residual = static_cast<const __half*>(a.residual);
-  p.M = a.M;
-  p.N = a.N;
-  p.K = a.K;
-  p.act = a.act;
+  p.out = a;
   p.tiles_m = (a.M + 128 * CG - 1) / (128 * CG);
   p.tiles_n = (a.N + BN - 1) / BN;
   p.stages = stages;
-  p.status = static_cast<int*>(ws);
+  p.splits = splits;
+  p.x_rows = x_rows;
   if (static_cast<long long>(p.tiles_m) * p.tiles_n > 0x3fffffffLL) return FG_ERR_SHAPE;
-  const int tiles = p.tiles_m * p.tiles_n, groups = tiles < dev.sm_count / CG ? tiles : dev.sm_count / CG;
+  const int cluster = CG * splits, tiles = p.tiles_m * p.tiles_n;
+  const int groups = splits > 1 || tiles < dev.sm_count / cluster ? tiles : dev.sm_count / cluster;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(groups * CG);
+  cfg.gridDim = dim3(groups * cluster);
   cfg.blockDim = dim3(fg::kGemm8Threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -130,35 +111,56 @@ int run_gemm(const Args& a, const fg::host::Device& dev, void* ws, cudaStream_t 
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = CG == 1 ? 1 : 2;
+  cfg.numAttrs = cluster == 1 ? 1 : 2;
   return fg::host::launched(cudaLaunchKernelEx(&cfg, kern, tmX, tmW, p));
 }
 
 }  // namespace
 
 extern "C" int fg_linear_w8a8(const int8_t* x8, const int8_t* W8, const void* x_scales, int x_scales_f32, const void* w_scales, void* C,
-                              int M, int N, int K, const void* bias, const void* residual, int act, void* ws, size_t ws_bytes,
+                              int M, int N, int K, const void* bias, const void* residual, int act, int* status_dev,
                               fg_stream_t stream) {
   if (x8 == nullptr || W8 == nullptr || C == nullptr || x_scales == nullptr) return FG_ERR_NULL;
   if (M <= 0 || N <= 0 || K <= 0 || (N % 128) != 0 || (K % 128) != 0 || K > kMaxK) return FG_ERR_SHAPE;
   if (act < FG_ACT_NONE || act > FG_ACT_SILU_GATE) return FG_ERR_PLAN;
   if (!aligned(x8, 16) || !aligned(W8, 16) || !aligned(C, 16) || !aligned(residual, 16) || !aligned(x_scales, x_scales_f32 ? 4 : 2) ||
-      !aligned(w_scales, 2) || !aligned(bias, 2))
+      !aligned(w_scales, 2) || !aligned(bias, 2) || !aligned(status_dev, 4))
     return FG_ERR_ALIGN;
-  if (ws == nullptr || !aligned(ws, 256) || ws_bytes < FG_WS_TICKETS_OFFSET + 4 * static_cast<size_t>(N / 128)) return FG_ERR_WORKSPACE;
   fg::host::Device dev;
   const int st = fg::host::current_device(&dev);
   if (st != FG_OK) return st;
-  const Args a = {x8, W8, x_scales, w_scales, x_scales_f32, C, M, N, K, bias, residual, act};
+  fg::W8A8Params a = {};
+  a.C = static_cast<__half*>(C);
+  a.x_scales = x_scales;
+  a.x_scales_f32 = x_scales_f32;
+  a.w_scales = static_cast<const __half*>(w_scales);
+  a.bias = static_cast<const __half*>(bias);
+  a.residual = static_cast<const __half*>(residual);
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.act = act;
+  a.status = status_dev;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (M <= fg::kGemv8MaxM) return run_gemv(a, s);
-  if (M <= kStreamRows) return run_streaming(a, dev, ws, s);
-  // Pairs of CTAs once their tiles fill the card, single CTAs with smaller tiles below.
-  const long long pair_tiles = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256);
-  if (2 * pair_tiles >= dev.sm_count) return run_gemm<2, 256>(a, dev, ws, s);
-  return run_gemm<1, 128>(a, dev, ws, s);
+  if (M <= fg::kGemv8MaxM) return run_gemv(a, x8, W8, s);
+  const Tiling t = choose_tiling(M, N, K, act == FG_ACT_SILU_GATE, dev.sm_count, dev.smem_optin);
+  if (t.cg == 2) return run_gemm<2, 256>(a, x8, W8, 1, dev, s);
+  switch (t.bn) {
+    case 32: return run_gemm<1, 32>(a, x8, W8, t.splits, dev, s);
+    case 64: return run_gemm<1, 64>(a, x8, W8, t.splits, dev, s);
+    case 96: return run_gemm<1, 96>(a, x8, W8, t.splits, dev, s);
+    case 128: return run_gemm<1, 128>(a, x8, W8, t.splits, dev, s);
+    case 192: return run_gemm<1, 192>(a, x8, W8, t.splits, dev, s);
+    default: return run_gemm<1, 256>(a, x8, W8, t.splits, dev, s);
+  }
+}
+
+// Internal (for the tests): the tiling of a call as bn | cg << 16 | splits << 24.
+extern "C" int fg_linear_w8a8_tiling(int M, int N, int K, int gated, int sm_count, int smem_optin) {
+  const Tiling t = choose_tiling(M, N, K, gated != 0, sm_count, smem_optin);
+  return t.bn | t.cg << 16 | t.splits << 24;
 }

@@ -140,55 +140,6 @@ static int aligned_grid(int tiles, int k_blocks, long long stage_bytes, int sm_c
   return 0;
 }
 
-// Ring and grid of the tcgen05 kernel for a plan whose m_tile and tiles are set.  extra_smem: bytes of shared memory the
-// launch needs beyond the ring.
-static int plan_umma(fg_plan_t* p, int op, int K, int max_grid, int sm_count, int smem_optin_bytes, int extra_smem) {
-  const int chunk_k = fg_chunk_k(op);
-  const int room = smem_optin_bytes - 1024 - 64 - extra_smem;
-  int chunks = 4;
-  while (chunks > 1 && chunks * chunk_k > K) chunks >>= 1;  // a stage never spans more than K
-  int stage_bytes = chunks * fg_chunk_bytes(op, p->m_tile);
-  p->stages = std::min(room / (stage_bytes + 16), FG_MAX_STAGES);
-  // Taller activation tiles: stages shrink one chunk at a time until the ring is three deep
-  // (measured at M = 32 / 64, 8192 x 8192: three chunks x 3 stages 26.9 / 30.6 us, two chunks
-  // x 5 / 4 stages 27.5 / 31.6 us, four chunks x 2 stages 27.0 / 30.7 us).
-  while (p->stages < 3 && chunks > 1) {
-    chunks -= 1;
-    stage_bytes = chunks * fg_chunk_bytes(op, p->m_tile);
-    p->stages = std::min(room / (stage_bytes + 16), FG_MAX_STAGES);
-  }
-  if (p->stages < 2) return FG_ERR_PLAN;
-  p->math = 2;
-  p->consumer_warps = 4;  // epilogue warps, fixed
-  p->k_per_stage = chunks * chunk_k;
-  p->k_blocks = (K + p->k_per_stage - 1) / p->k_per_stage;
-  const long long units = static_cast<long long>(p->tiles) * p->k_blocks;
-  p->grid = static_cast<int>(std::min<long long>(max_grid, units));
-  if (units * p->grid >= (1LL << 31)) return FG_ERR_SHAPE;
-  const int g = aligned_grid(p->tiles, p->k_blocks, static_cast<long long>(chunks) * FG_CHUNK_W_BYTES, sm_count);
-  if (g && g <= max_grid) p->grid = g;
-  p->pdl = 1;
-  p->smem_bytes = fg_umma_smem_bytes_mt(op, p->m_tile, chunks, p->stages) + extra_smem;
-  return FG_OK;
-}
-
-// int8 activations and weights: the tcgen05 kernel in the byte geometry of fp16 NxK weights, with up to 128 rows of
-// activations per pass.  Partial tiles of 128 rows are twice the size the workspace counts with: half as many CTAs.
-extern "C" int fg_plan_w8a8(int M, int N, int K, int sm_count, int smem_optin_bytes, int extra_smem_bytes, fg_plan_t* out) {
-  std::memset(out, 0, sizeof(*out));
-  if (M <= 0 || N <= 0 || K <= 0 || (N % 128) != 0 || (K % 128) != 0) return FG_ERR_SHAPE;
-  fg_plan_t p;
-  std::memset(&p, 0, sizeof(p));
-  p.op = FG_PLAN_OP_W8A8;
-  p.m_tile = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  p.passes = (M + 127) / 128;
-  p.tiles = N / 128;
-  const int max_grid = std::min(sm_count, p.m_tile == 128 ? FG_MAX_GRID / 2 : FG_MAX_GRID);
-  const int st = plan_umma(&p, FG_PLAN_OP_W8A8, K, max_grid, sm_count, smem_optin_bytes, extra_smem_bytes);
-  if (st == FG_OK) *out = p;
-  return st;
-}
-
 static int plan_impl(int op, int M, int N, int K, int sm_count, int smem_optin_bytes, fg_plan_t* out,
                      bool force_mma_sync, bool allow_gemv) {
   if (out == nullptr) return FG_ERR_NULL;
@@ -240,9 +191,37 @@ static int plan_impl(int op, int M, int N, int K, int sm_count, int smem_optin_b
     p.math = 2;
     if (p.m_tile < 16) p.m_tile = 16;  // rows beyond M are zero-filled by the TMA
     p.consumer_warps = 4;  // epilogue warps, fixed
-    const int st = plan_umma(&p, op, K, std::min(sm_count, FG_MAX_GRID), sm_count, smem_optin_bytes, 0);
-    if (st == FG_OK) *out = p;
-    return st;
+    int chunks = 4;
+    while (chunks > 1 && chunks * chunk_k > K) chunks >>= 1;  // a stage never spans more than K
+    p.k_per_stage = chunks * chunk_k;
+    p.k_blocks = (K + p.k_per_stage - 1) / p.k_per_stage;
+    const long long units = static_cast<long long>(p.tiles) * p.k_blocks;
+    p.grid = static_cast<int>(std::min<long long>(std::min(sm_count, FG_MAX_GRID), units));
+    if (units * p.grid >= (1LL << 31)) return FG_ERR_SHAPE;
+    int stage_bytes = chunks * fg_chunk_bytes(op, p.m_tile);
+    p.stages = std::min((smem_optin_bytes - 1024 - 64) / (stage_bytes + 16), FG_MAX_STAGES);
+    // Taller activation tiles: stages shrink one chunk at a time until the ring is three deep
+    // (measured at M = 32 / 64, 8192 x 8192: three chunks x 3 stages 26.9 / 30.6 us, two chunks
+    // x 5 / 4 stages 27.5 / 31.6 us, four chunks x 2 stages 27.0 / 30.7 us).
+    while (p.stages < 3 && chunks > 1) {
+      chunks -= 1;
+      p.k_per_stage = chunks * chunk_k;
+      p.k_blocks = (K + p.k_per_stage - 1) / p.k_per_stage;
+      stage_bytes = chunks * fg_chunk_bytes(op, p.m_tile);
+      p.stages = std::min((smem_optin_bytes - 1024 - 64) / (stage_bytes + 16), FG_MAX_STAGES);
+    }
+    if (p.stages < 2) return FG_ERR_PLAN;
+    {
+      const long long units2 = static_cast<long long>(p.tiles) * p.k_blocks;
+      p.grid = static_cast<int>(std::min<long long>(std::min(sm_count, FG_MAX_GRID), units2));
+      if (units2 * p.grid >= (1LL << 31)) return FG_ERR_SHAPE;
+      const int g = aligned_grid(p.tiles, p.k_blocks, static_cast<long long>(chunks) * FG_CHUNK_W_BYTES, sm_count);
+      if (g) p.grid = g;
+    }
+    p.pdl = 1;
+    p.smem_bytes = fg_umma_smem_bytes_mt(op, p.m_tile, chunks, p.stages);
+    *out = p;
+    return FG_OK;
   }
   if (quantized && p.m_tile == 16 && !force_mma_sync) {
     // Quantized weights, more than 8 token rows: warps dequantise landed stages into fp16 staging

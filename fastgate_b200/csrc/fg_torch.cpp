@@ -409,11 +409,16 @@ void hgemm_tr(at::Tensor A, at::Tensor W, at::Tensor C) {
 
 }  // namespace
 
-StreamWorkspace linear_workspace(int64_t device, cudaStream_t stream, int64_t N) {
-  const size_t bytes = fg_workspace_bytes(static_cast<int>(std::max<int64_t>(N, 65536)));
-  if (void* p = graph_workspace(static_cast<int>(device), stream, kLinearWorkspace, bytes)) return {at::Tensor(), p, bytes};
-  const Workspace w = workspace_for(static_cast<int>(device), stream, static_cast<int>(N));
-  return {w.buf, w.buf.data_ptr(), w.bytes};
+int* linear_status(int64_t device, cudaStream_t stream) {
+  {
+    // (a captured call only borrows what is there: the workspace's first use clears it, which is no work for a graph)
+    std::lock_guard<std::mutex> lk(g_ws_mu);
+    const auto w = g_ws.find({static_cast<int>(device), reinterpret_cast<int64_t>(stream)});
+    if (w != g_ws.end() && w->second.bytes > 0) return static_cast<int*>(w->second.buf.data_ptr());
+  }
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) return nullptr;
+  return static_cast<int*>(workspace_for(static_cast<int>(device), stream, 128).buf.data_ptr());
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

@@ -3,17 +3,11 @@
 #include <cuda_runtime.h>
 #include <torch/extension.h>
 
-enum WorkspaceKind { kLinearWorkspace = 0, kAttentionWorkspace = 1 };
 // The cleared workspace of a call that is being captured on `stream` (fg_torch_graph.cpp); nullptr: no capture.
-void* graph_workspace(int device, cudaStream_t stream, WorkspaceKind kind, size_t bytes);
-
-struct StreamWorkspace {
-  at::Tensor buf;   // keeps an eager call's memory alive
-  void* ptr = nullptr;
-  size_t bytes = 0;
-};
-// The linears' workspace for N output columns: of the (device, stream), or of the graph being captured (fg_torch.cpp).
-StreamWorkspace linear_workspace(int64_t device, cudaStream_t stream, int64_t N);
+void* graph_workspace(int device, cudaStream_t stream, size_t bytes);
+// The status word that workspace_status() reads: of the stream's workspace (fg_torch.cpp).  nullptr while the stream is
+// captured and has none yet.
+int* linear_status(int64_t device, cudaStream_t stream);
 
 // Operators around the linears of a serving step (fg_torch_serving.cpp).
 void bind_serving(pybind11::module& m);

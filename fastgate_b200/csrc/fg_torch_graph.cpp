@@ -10,7 +10,7 @@
 #include <map>
 #include <mutex>
 #include <stdexcept>
-#include <tuple>
+#include <utility>
 #include <vector>
 
 #include "fg_torch.h"
@@ -33,7 +33,7 @@ std::vector<Block>& blocks() {
   static std::vector<Block>* v = new std::vector<Block>;
   return *v;
 }
-using Key = std::tuple<unsigned long long, int64_t, int>;  // capture id, stream, kind
+using Key = std::pair<unsigned long long, int64_t>;  // capture id, stream
 std::map<Key, size_t>& taken() {
   static std::map<Key, size_t>* m = new std::map<Key, size_t>;
   return *m;
@@ -68,13 +68,13 @@ struct RelaxedMode {
 
 }  // namespace
 
-void* graph_workspace(int device, cudaStream_t stream, WorkspaceKind kind, size_t bytes) {
+void* graph_workspace(int device, cudaStream_t stream, size_t bytes) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   unsigned long long id = 0;
   cudaGraph_t graph = nullptr;
   must(cudaStreamGetCaptureInfo(stream, &status, &id, &graph));
   if (status != cudaStreamCaptureStatusActive) return nullptr;
-  const Key key{id, reinterpret_cast<int64_t>(stream), kind};
+  const Key key{id, reinterpret_cast<int64_t>(stream)};
   std::lock_guard<std::mutex> lk(mu());
   const auto known = taken().find(key);
   if (known != taken().end() && blocks()[known->second].bytes >= bytes) return blocks()[known->second].ptr;

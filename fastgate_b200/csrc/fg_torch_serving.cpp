@@ -171,13 +171,13 @@ void linear_int8(at::Tensor x8, at::Tensor W8, at::Tensor C, at::Tensor x_scales
     bad_argument("the output may be the residual itself; otherwise it must not overlap the inputs");
   const c10::cuda::CUDAGuard guard(x8.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
-  const StreamWorkspace ws = linear_workspace(device, stream, N);
+  int* status = linear_status(device, stream);
   int st;
   {
     pybind11::gil_scoped_release nogil;
     st = fg_linear_w8a8(static_cast<const int8_t*>(x8.data_ptr()), static_cast<const int8_t*>(W8.data_ptr()), x_scales.data_ptr(), f32, ws_ptr,
                         C.data_ptr(), static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), bias_ptr, res_ptr, code,
-                        ws.ptr, ws.bytes, reinterpret_cast<fg_stream_t>(stream));
+                        status, reinterpret_cast<fg_stream_t>(stream));
   }
   check_status(st);
 }
@@ -274,10 +274,14 @@ void kv_read_int4(at::Tensor pages, at::Tensor slots, at::Tensor k_out, at::Tens
 std::mutex g_attn_mu;
 std::map<std::pair<int64_t, int64_t>, at::Tensor> g_attn_ws;
 
+struct AttentionWorkspace {
+  at::Tensor buf;  // keeps an eager call's memory alive
+  void* ptr;
+};
 // One workspace per (device, stream), made on the first call, or the graph's own while one is captured.
-StreamWorkspace attention_workspace(int64_t device, cudaStream_t stream) {
+AttentionWorkspace attention_workspace(int64_t device, cudaStream_t stream) {
   const size_t bytes = fg_kv_attention_workspace_bytes();
-  if (void* p = graph_workspace(static_cast<int>(device), stream, kAttentionWorkspace, bytes)) return {at::Tensor(), p, bytes};
+  if (void* p = graph_workspace(static_cast<int>(device), stream, bytes)) return {at::Tensor(), p};
   std::lock_guard<std::mutex> lk(g_attn_mu);
   at::Tensor& t = g_attn_ws[{device, reinterpret_cast<int64_t>(stream)}];
   if (!t.defined()) {
@@ -285,7 +289,7 @@ StreamWorkspace attention_workspace(int64_t device, cudaStream_t stream) {
     check_status(fg_kv_attention_workspace_init(made.data_ptr(), bytes, reinterpret_cast<fg_stream_t>(stream)));
     t = made;
   }
-  return {t, t.data_ptr(), bytes};
+  return {t, t.data_ptr()};
 }
 
 void kv_attention_int4(at::Tensor q, at::Tensor pages, at::Tensor block_table, at::Tensor seq_lens, at::Tensor out, int64_t page_size,
@@ -326,14 +330,14 @@ void kv_attention_int4(at::Tensor q, at::Tensor pages, at::Tensor block_table, a
   if (B > 0x7fffffff || width > 0x7fffffff || T > 0x7fffffff / q_heads) bad_argument("too many rows");
   const c10::cuda::CUDAGuard guard(q.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
-  const StreamWorkspace ws = attention_workspace(device, stream);
+  const AttentionWorkspace ws = attention_workspace(device, stream);
   int st;
   {
     pybind11::gil_scoped_release nogil;
     st = fg_kv_attention_int4(q.data_ptr(), row_stride(q), out.data_ptr(), row_stride(out), T, static_cast<int>(q_heads),
                               static_cast<int>(heads), static_cast<int>(d), pages.data_ptr(), pages.size(0), static_cast<int>(page_size),
                               block_table.data_ptr<int>(), ldt, static_cast<int>(width), seq_lens.data_ptr<int>(), starts,
-                              static_cast<int>(B), static_cast<float>(sc), sp, ws.ptr, ws.bytes,
+                              static_cast<int>(B), static_cast<float>(sc), sp, ws.ptr, fg_kv_attention_workspace_bytes(),
                               reinterpret_cast<fg_stream_t>(stream));
   }
   check_status(st);

@@ -54,20 +54,6 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// int8 x int8 -> int32: the same operand geometry in bytes, 32 k per instruction.
-__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-template <int OP>
-__device__ __forceinline__ void umma_op(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (OP == kOpW8A8NK) umma_i8(tmem_d, adesc, bdesc, idesc, accumulate);
-  else umma_f16(tmem_d, adesc, bdesc, idesc, accumulate);
-}
 // The mbarrier gets one arrival when every MMA issued so far by this thread has completed.
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
@@ -98,10 +84,6 @@ __host__ __device__ constexpr uint64_t umma_smem_desc(uint32_t smem_addr, uint32
 __host__ __device__ constexpr uint32_t umma_idesc(bool a_mn_major, int n = kUmmaMT) {
   return (1u << 4) | ((a_mn_major ? 1u : 0u) << 15) | ((static_cast<uint32_t>(n) >> 3) << 17) | ((kTileN >> 4) << 24);
 }
-// Instruction descriptor, kind::i8: signed A and B, 32-bit integer D, both K-major.
-__host__ __device__ constexpr uint32_t umma_idesc_i8(int m, int n) {
-  return (2u << 4) | (1u << 7) | (1u << 10) | ((static_cast<uint32_t>(n) >> 3) << 17) | ((static_cast<uint32_t>(m) >> 4) << 24);
-}
 // 16 consecutive 32-bit columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -115,8 +97,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 // One output element of row m, column n (scale, round, store; push-aware like store_out2).
 template <int OP, int ACT>
 __device__ __forceinline__ void store_out1(const KParams& p, int m, int n, float v) {
-  v = scaled_sum<OP>(p, m, n, v);
-  if (ACT != kActNone || p.bias != nullptr || p.residual != nullptr) v = epilogue1<ACT, OP>(p, m, n, v);
+  if ((OP == kOpW8A16NK || (OP == kOpW4A16NK && p.scale_groups <= 1)) && p.scales != nullptr)
+    v *= __half2float(p.scales[n]);  // one scale per output channel, applied in fp32
+  if (ACT != kActNone || p.bias != nullptr || p.residual != nullptr) v = epilogue1<ACT>(p, m, n, v);
   const __half h = __float2half_rn(v);
   if (p.world == 0) {
     *out_ptr(p, m, n) = h;
@@ -133,15 +116,15 @@ __device__ __forceinline__ void store_out1(const KParams& p, int m, int n, float
   }
 }
 
-// MT = token rows of the accumulator = N of the MMA instruction: 16, 32 or 64 (int8 activations: 128 too, the whole
-// tensor memory).  Up to that many rows of activations ride along with one pass over the weight; the instruction count, and with it the
+// MT = token rows of the accumulator = N of the MMA instruction: 16, 32 or 64.  Up to 64 rows of
+// activations ride along with one pass over the weight; the instruction count, and with it the
 // issuing thread's time, does not depend on MT.
 template <int OP, int MT>
 __global__ void __launch_bounds__(kUmmaThreads, 1)
     fg_umma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                    const KParams p) {
-  static_assert(OP == kOpF16KN || OP == kOpF16NK || OP == kOpW8A8NK, "operands that the tensor core reads as they are");
-  static_assert(MT == 16 || MT == 32 || MT == 64 || (MT == 128 && OP == kOpW8A8NK), "accumulator height");
+  static_assert(OP == kOpF16KN || OP == kOpF16NK, "tcgen05 path: fp16 weights only");
+  static_assert(MT == 16 || MT == 32 || MT == 64, "accumulator height");
   using T = OpTraits<OP>;
   constexpr uint32_t kCols = 2 * kUmmaChains * MT;  // TMEM columns: 2 buffers x 2 chains x MT (64, 128 or 256)
   extern __shared__ uint8_t smem_raw[];
@@ -199,9 +182,6 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot_gen;
-  // the epilogue and finishing warps read row scales (and residuals) that the previous kernel may have written
-  if constexpr (OP == kOpW8A8NK)
-    if (warp != 4) griddep_wait();
 
   const uint32_t KB = p.k_blocks;
   const uint32_t total = static_cast<uint32_t>(p.tiles) * KB;
@@ -227,7 +207,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
     // them to the slot's empty barrier.  The mbarrier wait orders the TMA's writes before
     // the MMA's reads; tcgen05 fences are only needed around the accumulator hand-off.
     if (lane == 0) {
-      constexpr uint32_t idesc = OP == kOpW8A8NK ? umma_idesc_i8(kTileN, MT) : umma_idesc(OP == kOpF16KN, MT);
+      constexpr uint32_t idesc = umma_idesc(OP == kOpF16KN, MT);
       uint32_t u = ub;
       int it0 = 0;
       uint32_t sg = 0;
@@ -266,18 +246,18 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
           // K-major: a k16 step is 32 bytes further along the 128-byte rows (8-row groups
           // 1024 B apart).  MN-major: it is sixteen 128-byte k-rows = 2048 B further; the
           // two 64-column boxes are 8192 B apart (LBO), 8-row k-groups 1024 B (SBO).
-          constexpr uint64_t a_hi = (OP != kOpF16KN) ? umma_smem_desc(0, 1, 64) : umma_smem_desc(0, 512, 64);
+          constexpr uint64_t a_hi = (OP == kOpF16NK) ? umma_smem_desc(0, 1, 64) : umma_smem_desc(0, 512, 64);
           constexpr uint64_t b_hi = umma_smem_desc(0, 1, 64);
-          constexpr uint64_t a_step = (OP != kOpF16KN) ? 2 : 128;
+          constexpr uint64_t a_step = (OP == kOpF16NK) ? 2 : 128;
           uint32_t wb = smem_base + s * stage_bytes;
           uint32_t acc_flag = (it > it0) ? 1u : 0u;
           for (int c = 0; c < nch; ++c) {
             const uint64_t a0 = a_hi | (wb >> 4);
             const uint64_t b0 = b_hi | ((wb + kChunkWBytes) >> 4);
-            umma_op<OP>(tmem_d, a0, b0, idesc, acc_flag);
-            umma_op<OP>(tmem_d + MT, a0 + a_step, b0 + 2, idesc, acc_flag);
-            umma_op<OP>(tmem_d, a0 + 2 * a_step, b0 + 4, idesc, 1u);
-            umma_op<OP>(tmem_d + MT, a0 + 3 * a_step, b0 + 6, idesc, 1u);
+            umma_f16(tmem_d, a0, b0, idesc, acc_flag);
+            umma_f16(tmem_d + MT, a0 + a_step, b0 + 2, idesc, acc_flag);
+            umma_f16(tmem_d, a0 + 2 * a_step, b0 + 4, idesc, 1u);
+            umma_f16(tmem_d + MT, a0 + 3 * a_step, b0 + 6, idesc, 1u);
             acc_flag = 1u;
             wb += cbytes;
           }
@@ -332,22 +312,14 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
             tmem_ld32(tbase, q);
             tmem_ld_wait();
 #pragma unroll
-            for (int m = 0; m < 16; ++m) {
-              float v = __uint_as_float(q[m]);
-              add_sum<OP>(v, __uint_as_float(q[16 + m]));
-              r[m] = __float_as_uint(v);
-            }
+            for (int m = 0; m < 16; ++m) r[m] = __float_as_uint(__uint_as_float(q[m]) + __uint_as_float(q[16 + m]));
           } else {
             uint32_t q0[16], q1[16];
             tmem_ld16(tbase + mg * 16, q0);
             tmem_ld16(tbase + MT + mg * 16, q1);
             tmem_ld_wait();
 #pragma unroll
-            for (int m = 0; m < 16; ++m) {
-              float v = __uint_as_float(q0[m]);
-              add_sum<OP>(v, __uint_as_float(q1[m]));
-              r[m] = __float_as_uint(v);
-            }
+            for (int m = 0; m < 16; ++m) r[m] = __float_as_uint(__uint_as_float(q0[m]) + __uint_as_float(q1[m]));
           }
           if (mg == MT / 16 - 1) {
             tc_fence_before_sync();
@@ -369,7 +341,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1)
 #pragma unroll
             for (int m = 0; m < 16; ++m)
               if (mg * 16 + m < p.M)
-                store_gate<OP>(p, mg * 16 + m, tile, n_in_tile, __uint_as_float(r[m]), gate_xch[m * kTileN + 64 + n_in_tile]);
+                store_gate(p, mg * 16 + m, tile, n_in_tile, __uint_as_float(r[m]), gate_xch[m * kTileN + 64 + n_in_tile]);
           }
           named_bar_sync(1, 128);
         } else if (whole) {

@@ -1,4 +1,4 @@
-"""linear_int8 against 64 bits: streaming and paired kernels, every epilogue, the largest sums, splits and graphs."""
+"""linear_int8 against 64 bits: the GEMV and every tiling of the tensor-core kernel, every epilogue, the largest sums, graphs."""
 import ctypes
 
 import pytest
@@ -85,8 +85,8 @@ def test_largest_sums(M, dev):
 
 
 def test_rows_do_not_depend_on_their_company(dev):
-    """Exact sums and the same roundings after them: row i of every path (GEMV, streaming with each tile height, single CTAs,
-    pairs) has the same bits, whatever the epilogue."""
+    """Exact sums and the same roundings after them: row i of every path (GEMV, tiles of each width, clusters that share k, pairs)
+    has the same bits, whatever the epilogue."""
     x, w, sx, sw, g = _data(2600, 8192, 384, 11)
     xd, wd, sxd, swd = x.to(dev), w.to(dev), sx.to(dev), sw.to(dev)
     bias, res = torch.randn(8192, generator=g).half().to(dev), torch.randn(2600, 8192, generator=g).half().to(dev)
@@ -132,7 +132,8 @@ def test_gate_from_two_weights(M, dev):
 
 @pytest.mark.parametrize("M", [8, 100, 160, 2048])
 def test_two_graphs_of_one_stream_side_by_side(M, dev):
-    """Graphs captured on one stream have workspaces of their own: replayed on two streams at once they do not meet."""
+    """Graphs captured on one stream, replayed on two streams at once, do not meet (the operator keeps nothing between its CTAs
+    but a cluster's shared memory)."""
     x, w, sx, sw, _ = _data(M, 4096, 2048, 21)
     xd, wd, sxd, swd = x.to(dev), w.to(dev), sx.to(dev), sw.to(dev)
     want = torch.empty(M, 4096, dtype=torch.half, device=dev)
@@ -205,7 +206,6 @@ def test_refusals(dev):
     both = torch.empty(2 * 128 + 128, dtype=torch.half, device=dev)
     with pytest.raises(ValueError):  # the residual one row further in the same buffer
         fg.linear_int8(x, w, both[:256].view(2, 128), s, residual=both[128:].view(2, 128))
-    L, ws = capi.lib, torch.empty(capi.workspace_bytes(128), dtype=torch.uint8, device=dev)
-    args = lambda act=0, wsb=ws.numel(): L.fg_linear_w8a8(x.data_ptr(), w.data_ptr(), s.data_ptr(), 1, None, c.data_ptr(), 2, 128, 256, None,
-                                                          None, act, ws.data_ptr(), wsb, ctypes.c_void_p(0))
-    assert args(act=9) == capi.FG_ERR_PLAN and args(wsb=1024) == capi.FG_ERR_WORKSPACE
+    args = lambda act=0, xs=s.data_ptr(): capi.lib.fg_linear_w8a8(x.data_ptr(), w.data_ptr(), xs, 1, None, c.data_ptr(), 2, 128, 256, None, None, act,
+                                                                  None, ctypes.c_void_p(0))
+    assert args(act=9) == capi.FG_ERR_PLAN and args(xs=None) == capi.FG_ERR_NULL

@@ -21,13 +21,11 @@ def test_norm_arguments():
 
 
 def test_linear_arguments():
-    wsb = capi.workspace_bytes(128)
-    call = lambda x=P, w=P, s=P, c=P, M=1, N=128, K=128, res=None, act=0, ws=P, wsb=wsb: L.fg_linear_w8a8(x, w, s, 1, None, c, M, N, K, None, res, act, ws, wsb, None)
+    call = lambda x=P, w=P, s=P, c=P, M=1, N=128, K=128, res=None, act=0, st=None: L.fg_linear_w8a8(x, w, s, 1, None, c, M, N, K, None, res, act, st, None)
     assert call(x=None) == call(w=None) == call(s=None) == call(c=None) == capi.FG_ERR_NULL
     assert call(M=0) == call(N=100) == call(K=64) == call(K=131072) == capi.FG_ERR_SHAPE
     assert call(act=5) == call(act=-1) == capi.FG_ERR_PLAN
-    assert call(x=P + 8) == call(c=P + 8) == call(res=P + 2) == call(s=P + 2) == capi.FG_ERR_ALIGN
-    assert call(ws=None) == call(ws=P + 16) == call(wsb=4096) == capi.FG_ERR_WORKSPACE
+    assert call(x=P + 8) == call(c=P + 8) == call(res=P + 2) == call(s=P + 2) == call(st=P + 1) == capi.FG_ERR_ALIGN
 
 
 def test_cache_arguments():
@@ -56,7 +54,7 @@ def test_valid_arguments_stop_at_the_device():
     if torch.cuda.is_available():
         pytest.skip("a device is there: host addresses would be used")
     assert L.fg_add_rmsnorm(P, 64, P, None, None, 0, P, 0, None, 2, 64, 1e-6, None) == capi.FG_ERR_NO_DEVICE
-    assert L.fg_linear_w8a8(P, P, P, 1, None, P, 1, 128, 128, None, None, 0, P, capi.workspace_bytes(128), None) == capi.FG_ERR_NO_DEVICE
+    assert L.fg_linear_w8a8(P, P, P, 1, None, P, 1, 128, 128, None, None, 0, None, None) == capi.FG_ERR_NO_DEVICE
     assert L.fg_kv_read_int4(P, 4, 16, 2, 64, P, 1, 1, P, P, None, None) == capi.FG_ERR_NO_DEVICE
 
 
@@ -99,15 +97,21 @@ def test_rotation_table_keeps_far_angles():
     assert float((t[200000].double() - torch.cat([a.cos(), a.sin()])).abs().max()) <= 2.0 ** -24
 
 
-def test_plan_of_the_streaming_kernel_fits():
-    """Every plan for int8 activations leaves the ring at least two deep, within shared memory and the partial tiles' room."""
-    p = capi.Plan()
-    for M in (1, 16, 17, 32, 33, 64, 65, 128):
-        for N, K in ((128, 128), (4096, 4096), (28672, 8192), (256, 130944), (65536, 384)):
-            for extra in (0, 8192):
-                assert L.fg_plan_w8a8(M, N, K, 148, 232448, extra, ctypes.byref(p)) == capi.FG_OK
-                assert p.m_tile >= min(M, 128) and p.passes == 1 and p.stages >= 2 and p.smem_bytes <= 232448
-                assert p.k_per_stage % 128 == 0 and p.k_blocks * p.k_per_stage >= K > (p.k_blocks - 1) * p.k_per_stage
-                assert 1 <= p.grid <= 148 and p.grid * 2 * p.m_tile * 128 * 4 <= 256 * 2 * 64 * 128 * 4
-                assert p.smem_bytes >= 1024 + p.stages * ((p.k_per_stage // 128) * (16384 + 128 * p.m_tile) + 16) + 64 + extra
-    assert L.fg_plan_w8a8(1, 100, 128, 148, 232448, 0, ctypes.byref(p)) == capi.FG_ERR_SHAPE
+def test_tilings_of_the_linear_are_launchable():
+    """Every choice: a known tile, a cluster only where its tiles fit the card at once, no CTA without a stage of k, the
+    followers' sums within the leader's ring."""
+    blocks = {32: 2, 64: 2, 96: 2, 128: 2, 192: 1, 256: 1}
+    for M in (3, 16, 17, 64, 100, 128, 129, 300, 1000, 3001, 8192):
+        for N in (128, 512, 640, 1024, 4096, 11008, 28672, 65536):
+            for K in (128, 256, 384, 2048, 4096, 11008, 130944):
+                for gated in (0, 1):
+                    t = L.fg_linear_w8a8_tiling(M, N, K, gated, 148, 232448)
+                    bn, cg, splits = t & 0xFFFF, t >> 16 & 0xFF, t >> 24
+                    assert bn in blocks and (cg, splits) in ((1, 1), (1, 2), (1, 4), (1, 8), (2, 1)) and (cg == 1 or bn == 256)
+                    assert not gated or bn not in (96, 192)
+                    if splits > 1:
+                        tiles = -(-M // 128) * -(-N // bn)
+                        per = blocks[bn]
+                        stage = per * (128 + bn) * 128
+                        ring = (232448 - 1024 - 64 - 8 * bn) // (stage + 16) * stage
+                        assert tiles * splits <= 148 - 148 // 8 and -(-K // 128 // per) >= splits and (splits - 1) * bn * 512 <= ring
