@@ -36,10 +36,7 @@ struct Gemm8Params {
 };
 
 __host__ __device__ constexpr int gemm8_block_bytes(int cg, int bn) { return (128 + bn / cg) * 128; }
-// Accumulation chains of a tile: consecutive MMAs into one accumulator wait for each other; tiles that leave tensor memory
-// free deal the k steps to two or four accumulators, which the epilogue adds up (exactly: integers).
-__host__ __device__ constexpr int gemm8_chains(int bn) { return bn <= 64 ? 4 : bn <= 128 ? 2 : 1; }
-__host__ __device__ constexpr uint32_t gemm8_tmem_cols(int bn) { return bn * gemm8_chains(bn) <= 128 ? 256 : 512; }
+__host__ __device__ constexpr uint32_t gemm8_tmem_cols(int bn) { return bn <= 32 ? 64 : bn <= 64 ? 128 : bn <= 128 ? 256 : 512; }  // two accumulators
 // Weight rows of one copy: with the SiLU gate a tile narrower than a block of 128 takes gate rows and up rows separately.
 __host__ __device__ constexpr int gemm8_box_rows(int cg, int bn, bool gated) { return gated && bn / cg < 128 ? bn / 2 : bn / cg; }
 // k blocks of 128 that a stage holds: the barrier traffic around a stage costs its two threads as much as the copies and MMAs
@@ -125,31 +122,21 @@ __device__ __forceinline__ void gemm8_commit(uint32_t bar) {
   }
 }
 
-// kPiece columns of this thread's TMEM lane, the chains added up.
-template <int BN, int CHAINS, int PIECE>
-__device__ __forceinline__ void load_sums(uint32_t tbase, int col, uint32_t (&r)[PIECE]) {
-  uint32_t part[CHAINS][PIECE];
-#pragma unroll
-  for (int i = 0; i < CHAINS; ++i) {
-    if constexpr (PIECE == 32) tmem_ld32(tbase + i * BN + col, part[i]);
-    else tmem_ld16(tbase + i * BN + col, part[i]);
-  }
+// PIECE columns of this thread's TMEM lane.
+template <int PIECE>
+__device__ __forceinline__ void load_sums(uint32_t taddr, uint32_t (&r)[PIECE]) {
+  if constexpr (PIECE == 32) tmem_ld32(taddr, r);
+  else tmem_ld16(taddr, r);
   tmem_ld_wait();
-#pragma unroll
-  for (int j = 0; j < PIECE; ++j) {
-    r[j] = part[0][j];
-#pragma unroll
-    for (int i = 1; i < CHAINS; ++i) r[j] += part[i][j];
-  }
 }
 
 template <int CG, int BN>
 __global__ void __launch_bounds__(kGemm8Threads, 1)
     fg_gemm8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const Gemm8Params p) {
   constexpr int kBlock = gemm8_block_bytes(CG, BN), kPer = gemm8_blocks_per_stage(CG, BN), kStage = kPer * kBlock;
-  constexpr uint32_t kCols = gemm8_tmem_cols(BN);  // two accumulators of BN columns
-  constexpr int kChains = gemm8_chains(BN);
-  static_assert(2 * kChains * BN <= static_cast<int>(kCols), "tensor memory");
+  constexpr uint32_t kCols = gemm8_tmem_cols(BN);
+  constexpr int kPiece = BN >= 64 ? 32 : 16;       // columns that the epilogue takes at a time
+  static_assert(2 * BN <= static_cast<int>(kCols), "tensor memory");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -213,10 +200,9 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
     const W8A8Params& q = p.out;
     const int width = gated ? q.N >> 1 : q.N;
     if (!__any_sync(0xffffffffu, row)) return;  // a small M: nothing to store for these rows
-    constexpr int kPiece = kChains <= 2 ? 32 : 16;
-    const uint32_t tbase = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + b * kChains * BN;
+    const uint32_t tbase = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + b * BN;
     auto load_piece = [&](int col, uint32_t (&r)[kPiece]) {
-      load_sums<BN, kChains, kPiece>(tbase, col, r);
+      load_sums(tbase + col, r);
       if (CG == 1 && more != nullptr)
         for (int i = 0; i < splits - 1; ++i)
 #pragma unroll
@@ -375,7 +361,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
           break;
         }
         tc_fence_after_sync();
-        const uint32_t acc = tmem_base + b * kChains * BN;
+        const uint32_t acc = tmem_base + b * BN;
         for (int ks = ks0; ks < ks1; ++ks) {
           if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar_full + 8 * s, ph, kWaitBudgetNs))) {
             dead = true;
@@ -388,8 +374,8 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
               if (i == 0 || ks * kPer + i < k_blocks) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  gemm8_mma<CG>(acc + k % kChains * BN, at + (i * kBlock / 16 + 2 * k), at + ((i * kBlock + 16384) / 16 + 2 * k), idesc,
-                                ks != ks0 || i != 0 || k >= kChains);
+                  gemm8_mma<CG>(acc, at + (i * kBlock / 16 + 2 * k), at + ((i * kBlock + 16384) / 16 + 2 * k), idesc,
+                                ks != ks0 || i != 0 || k != 0);
               }
             }
             gemm8_commit<CG>(bar_empty + 8 * s);
@@ -451,11 +437,10 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
       const uint32_t sums = smem_base;
       if (warp < 4 && part > 0) {
         const uint32_t to = map_to_rank(sums, 0) + (((part - 1) * BN) * 128 + 32 * warp + lane) * 4;
-        constexpr int kPiece = kChains <= 2 ? 32 : 16;
 #pragma unroll 1
         for (int c = 0; c < BN; c += kPiece) {
           uint32_t r[kPiece];
-          load_sums<BN, kChains, kPiece>(tmem_base + (static_cast<uint32_t>(warp * 32) << 16), c, r);
+          load_sums(tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + c, r);
 #pragma unroll
           for (int j = 0; j < kPiece; ++j) st_cluster(to + (c + j) * 512, r[j]);
         }

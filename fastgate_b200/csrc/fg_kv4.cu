@@ -306,9 +306,10 @@ extern "C" int fg_kv_append_int4(const void* k, long long ldk, const void* v, lo
   p.kv = {static_cast<uint8_t*>(pages), num_pages, kv_heads, page_size};
   p.status = status_dev;
   p.tokens = tokens;
-  // Few rows: one a lane group, for latency; enough rows to fill the card twice over: four.
+  // Few rows: one a lane group, for latency; enough rows for two CTAs' worth a SM with four: four (6001 tokens of 48 heads of
+  // 64 channels: 17.7 us against 19.9).
   const long long heads = q_heads + 2LL * kv_heads, rows_per_cta = kKvThreads / (d / 16);
-  const bool many = tokens * heads >= 4 * 8 * rows_per_cta * dev.sm_count;
+  const bool many = tokens * heads >= 4 * 4 * rows_per_cta * dev.sm_count;
   const long long gx = (tokens + rows_per_cta - 1) / rows_per_cta, gy = (heads + (many ? 3 : 0)) / (many ? 4 : 1);
   if (gx > 0x7fffffffLL || gy > 65535) return FG_ERR_SHAPE;
   void (*kern)(const AppendParams) = d == 128 ? (many ? fg_kv_append_kernel<128, 4> : fg_kv_append_kernel<128, 1>)
@@ -336,7 +337,7 @@ extern "C" int fg_kv_read_int4(const void* pages, long long num_pages, int page_
   p.status = status_dev;
   p.tokens = tokens;
   const long long rows_per_cta = kKvThreads / (d / 8), gx = (tokens + rows_per_cta - 1) / rows_per_cta;
-  const bool many = tokens * kv_heads >= 4 * 8 * rows_per_cta * dev.sm_count;
+  const bool many = tokens * kv_heads >= 4 * 8 * rows_per_cta * dev.sm_count;  // 40000 rows: 38 us, with one head a thread 47
   const long long gy = (kv_heads + (many ? 3 : 0)) / (many ? 4 : 1);
   if (gx > 0x7fffffffLL || gy > 65535) return FG_ERR_SHAPE;
   void (*kern)(const ReadParams) = d == 128 ? (many ? fg_kv_read_kernel<128, 4> : fg_kv_read_kernel<128, 1>)
