@@ -17,10 +17,18 @@
 //     movmatrix makes the second product's operand; nothing goes through shared memory but the cache itself.
 //     (tcgen05.mma takes its operands from shared memory: the codes would have to be written back there as fp16, four
 //     times the bytes that came in.)
-//   - The softmax's running maximum moves only when a weight exceeds it by more than 2^8 (a warp vote per 32 rows instead
+//   - The softmax's running maximum moves only when a weight exceeds it by more than 2^8 (a warp vote per 32 or 64 rows instead
 //     of a reduction); weights then stay below 2^8 and exact sums are unchanged, since every term uses the same m.
 //     The maximum is taken over log2(p_t sv_t), the weight that is rounded to fp16: its relative error is 2^-11 whatever
 //     the scale of the values.
+//   - The fp16 weights alone would leave the output's error at 2.7 times that of an exact result rounded to fp16 (codes are never
+//     negative, so errors of weights meet codes at their full size).  What the rounding of a weight leaves over, again in fp16, is
+//     a second operand of the same product: 1.00 to 1.2 times then.  (64 sequences of up to 8000 rows: 95 us against 86
+//     without; the weights' errors on codes about their middle, which costs 88, still give 1.4 to 1.55.)
+//   - The tensor core cuts off, towards zero, what does not fit below a 32-bit accumulator; over thousands of rows of
+//     codes that are never negative that adds up (3.3 times the rounding of the output).  Every kDriftSlots slots one more product
+//     takes 7.5 times the weights of those slots off all accumulators, halfway, and its exact amount goes to the 32-bit sums:
+//     the accumulators stay small, and are below zero as often as above.
 //
 // Each warp streams its own slots of four blocks through its own ring (bulk copies, one mbarrier per slot), so no
 // warp waits for another inside a segment.  The rows of all (sequence, head, query tile) items form one list of 256-row
@@ -40,11 +48,12 @@ namespace {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
-constexpr int kPairRows = 2 * kKvBlock;       // rows that one step of the softmax takes
+constexpr int kPairRows = 2 * kKvBlock;       // rows of one masked step of the softmax
 constexpr int kSlotBlocks = 4;                // blocks of a ring slot
 constexpr int kSlotRows = kSlotBlocks * kKvBlock;
 constexpr int kUnitRows = kAttnWarps * kSlotRows;
 constexpr int kAttnMaxGrid = 1024;
+constexpr int kDriftSlots = 4;                // slots of a warp per correction (8 gave up to 1.4 times the output's rounding)
 constexpr float kLazyMax = 8.f;               // log2 of how far a weight may exceed the running maximum
 constexpr float kNoMax = -1e30f;              // stands for the maximum of no rows (scores stay far above it)
 constexpr float kMaxScale = 1048576.f;        // largest softmax scale: |scores| < 2^20 * 128 * 2^36
@@ -60,9 +69,10 @@ __host__ __device__ constexpr int attn_slot_bytes(int d, int cols) {            
   return kSlotBlocks * kv_block_bytes(d) > cols * d * 4 ? kSlotBlocks * kv_block_bytes(d) : cols * d * 4;
 }
 __host__ __device__ constexpr int attn_smem_bytes(int d, int cols) { return kAttnWarps * attn_stages(d) * attn_slot_bytes(d, cols); }
-// What the registers allow without spilling: 165 with eight columns, 255 with sixteen.  (Measured, 64 sequences of up to 8000
-// rows, eight columns, two / three / four CTAs: 119 / 86 / 88 us; 24 x 3000 rows of 64 channels, sixteen columns: 20.6 / 22.9 / 28.4.)
-__host__ __device__ constexpr int attn_ctas_per_sm(int cols) { return cols == 8 ? 3 : 2; }
+// (Measured with eight columns, two CTAs that take four blocks a step / three that have registers for two: 64 sequences of up to
+// 8000 rows 95 / 99 us, one of 5000 11.1 / 13.7.  A third ring slot changes neither.  Sixteen columns, 24 x 3000 rows of 64
+// channels, two / three / four CTAs: 20.6 / 22.9 / 28.4, before the second operand of the weights.)
+constexpr int kAttnCtasPerSm = 2;
 constexpr int kAttnMaxCols = 16;
 
 struct AttnParams {
@@ -183,7 +193,7 @@ struct Pending {
 };
 
 template <int D, int NQ>
-__global__ void __launch_bounds__(kAttnThreads, attn_ctas_per_sm(8 * NQ)) fg_kv_attention_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) fg_kv_attention_kernel(const AttnParams p) {
   constexpr int COLS = 8 * NQ;          // query columns of an item
   constexpr int KW = D / 32;            // 32-bit words of a key row per lane
   constexpr int VW = D / 64;            // 32-bit words of a value row per lane
@@ -409,8 +419,10 @@ __global__ void __launch_bounds__(kAttnThreads, attn_ctas_per_sm(8 * NQ)) fg_kv_
     const int min_limit = sq.len - sq.nq + (tile * COLS) / p.group;  // column 0 sees least
 
     float oacc[NQ][MT][4], mref[NQ][2], lsum[NQ][2], zsum[NQ][2];
+    __half2 drift[NQ];  // weights of up to kDriftSlots slots: 2^8 * 2 * 16 at most
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
+      drift[n] = __float2half2_rn(0.f);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         mref[n][i] = 0.f;
@@ -427,14 +439,15 @@ __global__ void __launch_bounds__(kAttnThreads, attn_ctas_per_sm(8 * NQ)) fg_kv_
     const int ka = (g & 1) ? 4 + ((g >> 1) ^ 1) : g >> 1;
     const int v0 = c, v1 = 4 + (c ^ 1);
     bool fresh = true;  // no rows yet: the first ones set the maximum, whatever its size
-    // Two blocks.  MASKED: some column does not see all of their rows, or a block is absent.
-    auto consume = [&](const uint8_t* base, int row0, uint32_t absent, auto masked_tag) {
+    // NB blocks.  MASKED: some column does not see all of their rows, or a block is absent.
+    auto consume = [&](const uint8_t* base, int row0, uint32_t absent, auto masked_tag, auto blocks_tag) {
       constexpr bool MASKED = decltype(masked_tag)::value;
-      float t[2][NQ][4];         // log2 of the weights over the values' scales, less the running maximum
-      float sv[2][2], lv[2][2];  // the value rows' scale and low end
+      constexpr int NB = decltype(blocks_tag)::value;
+      float t[NB][NQ][4];          // log2 of the weights over the values' scales, less the running maximum
+      float sv[NB][2], lv[NB][2];  // the value rows' scale and low end
       bool up = fresh;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < NB; ++h) {
         const uint8_t* blk = base + h * SB;
         // S^T = K Q^T on the codes
         uint32_t wa[KW], wb[KW];
@@ -474,12 +487,13 @@ __global__ void __launch_bounds__(kAttnThreads, attn_ctas_per_sm(8 * NQ)) fg_kv_
       if (__any_sync(0xffffffffu, up)) {
         // a new maximum: the largest of the old one and these rows', and everything so far brought to it
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+        for (int n = 0; n < NQ; ++n) {
+          drift[n] = __float2half2_rn(0.f);  // what they added has just shrunk
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             float m = fresh ? -INFINITY : 0.f;  // relative to the old one
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < NB; ++h)
 #pragma unroll
               for (int r = 0; r < 2; ++r) m = fmaxf(m, t[h][n][2 * r + q] + lg2(fmaxf(sv[h][r], 5.9604644775390625e-8f)));
 #pragma unroll
@@ -490,7 +504,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_ctas_per_sm(8 * NQ)) fg_kv_
             lsum[n][q] *= f;
             zsum[n][q] *= f;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < NB; ++h) {
               t[h][n][q] -= m;
               t[h][n][2 + q] -= m;
             }
@@ -500,12 +514,13 @@ __global__ void __launch_bounds__(kAttnThreads, attn_ctas_per_sm(8 * NQ)) fg_kv_
               oacc[n][i][2 + q] *= f;
             }
           }
-        if (absent != 3u) fresh = false;
+        }
+        if (absent != (1u << NB) - 1) fresh = false;
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < NB; ++h) {
         const uint8_t* blk = base + h * SB;
-        uint32_t pb[NQ][2];
+        uint32_t pb[NQ][2], pl[NQ][2];  // the weights' fp16, and what it leaves over
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
           float wgt[4];
@@ -522,8 +537,13 @@ __global__ void __launch_bounds__(kAttnThreads, attn_ctas_per_sm(8 * NQ)) fg_kv_
             }
           }
           const __half2 h0 = __floats2half2_rn(wgt[0], wgt[1]), h1 = __floats2half2_rn(wgt[2], wgt[3]);
+          const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+          const __half2 l0 = __floats2half2_rn(wgt[0] - f0.x, wgt[1] - f0.y), l1 = __floats2half2_rn(wgt[2] - f1.x, wgt[3] - f1.y);
+          drift[n] = __hadd2(drift[n], __hadd2(h0, h1));
           pb[n][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&h0));
           pb[n][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&h1));
+          pl[n][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&l0));
+          pl[n][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&l1));
         }
         // O^T += V^T P^T on the codes: lane g owns channels 8 VW g.., operand columns are rows (v0, v1) and (v0, v1) + 8
         uint32_t r0[VW], r1[VW], r2[VW], r3[VW];
@@ -537,20 +557,23 @@ __global__ void __launch_bounds__(kAttnThreads, attn_ctas_per_sm(8 * NQ)) fg_kv_
           for (int hf = 0; hf < 2; ++hf) {
             // row g: the even channel's code; row g + 8: the whole byte, even + 16 odd (an exact fp16 too), which takes no
             // second mask: the odd channel's sum is the difference, once at the end
-            uint32_t xa = prmt(r0[i], r1[i], hf ? 0x7632 : 0x5410), xb = prmt(r2[i], r3[i], hf ? 0x7632 : 0x5410);
+            const uint32_t xa = prmt(r0[i], r1[i], hf ? 0x7632 : 0x5410), xb = prmt(r2[i], r3[i], hf ? 0x7632 : 0x5410);
+            const uint32_t ya[2] = {xa & 0x00FF00FFu, prmt(xa, 0u, 0x4341)}, yb[2] = {xb & 0x00FF00FFu, prmt(xb, 0u, 0x4341)};
 #pragma unroll
-            for (int by = 0; by < 2; ++by) {
-              const uint32_t ya = by ? prmt(xa, 0u, 0x4341) : xa & 0x00FF00FFu, yb = by ? prmt(xb, 0u, 0x4341) : xb & 0x00FF00FFu;
+            for (int part = 0; part < 2; ++part)
 #pragma unroll
-              for (int n = 0; n < NQ; ++n) {
-                float* o = oacc[n][i * 4 + hf * 2 + by];
-                mma_codes(oacc[n][i * 4 + hf * 2 + by], ya & 0x000F000Fu, ya, yb & 0x000F000Fu, yb, pb[n][0], pb[n][1], o[0], o[1], o[2], o[3]);
-              }
-            }
+              for (int by = 0; by < 2; ++by)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                  float* o = oacc[n][i * 4 + hf * 2 + by];
+                  mma_codes(oacc[n][i * 4 + hf * 2 + by], ya[by] & 0x000F000Fu, ya[by], yb[by] & 0x000F000Fu, yb[by],
+                            part ? pl[n][0] : pb[n][0], part ? pl[n][1] : pb[n][1], o[0], o[1], o[2], o[3]);
+                }
           }
       }
     };
 
+    constexpr int kStep = 4 / NQ;  // blocks of one softmax step, as registers allow
     int row0 = (seg.first * kAttnWarps + warp) * kSlotRows;
     for (int j = 0; j < n_slots; ++j, row0 += kUnitRows) {
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar + 8 * slot, (phase >> slot) & 1u, kAttnWaitNs))) {
@@ -563,13 +586,32 @@ __global__ void __launch_bounds__(kAttnThreads, attn_ctas_per_sm(8 * NQ)) fg_kv_
       const uint32_t absent = (gone >> (kSlotBlocks * slot)) & kSlotMask;
       if (row0 + kSlotRows - 1 <= min_limit && absent == 0) {
 #pragma unroll
-        for (int h = 0; h < kSlotBlocks / 2; ++h) consume(base + h * (2 * SB), 0, 0u, std::false_type{});
+        for (int h = 0; h < kSlotBlocks; h += kStep) consume(base + h * SB, 0, 0u, std::false_type{}, std::integral_constant<int, kStep>{});
       } else {
 #pragma unroll 1
         for (int h = 0; h < kSlotBlocks / 2; ++h)
-          if (row0 + h * kPairRows < sq.len) consume(base + h * (2 * SB), row0 + h * kPairRows, (absent >> (2 * h)) & 3u, std::true_type{});
+          if (row0 + h * kPairRows < sq.len) consume(base + h * (2 * SB), row0 + h * kPairRows, (absent >> (2 * h)) & 3u, std::true_type{}, std::integral_constant<int, 2>{});
       }
       __syncwarp();  // every lane has read the slot
+      if (j % kDriftSlots == kDriftSlots - 1) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) drift[n] = __float2half2_rn(0.f);
+      }
+      if (j % kDriftSlots == kDriftSlots / 2 - 1) {  // for what these two slots have added and as much that is to come
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          const __half2 off = __hneg2(drift[n]);  // times code 15 of either nibble
+          const float2 f = __half22float2(off);
+          zsum[n][0] = fmaf(-15.f, f.x, zsum[n][0]);
+          zsum[n][1] = fmaf(-15.f, f.y, zsum[n][1]);
+          const uint32_t b = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&off));
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            float* o = oacc[n][t];
+            mma_codes(oacc[n][t], 0x000F000Fu, 0x00FF00FFu, 0u, 0u, b, 0u, o[0], o[1], o[2], o[3]);
+          }
+        }
+      }
       if (j + 1 < n_slots) copy_next();  // (the last one's is parked in first)
       slot = slot + 1 == S ? 0 : slot + 1;
     }
@@ -797,6 +839,6 @@ extern "C" int fg_kv_attention_int4(const void* q, long long ldq, void* out, lon
                                    : (cols == 16 ? fg_kv_attention_kernel<64, 2> : fg_kv_attention_kernel<64, 1>);
   const int smem = attn_smem_bytes(d, cols);
   if ((st = host::opt_in_smem(reinterpret_cast<const void*>(kern), smem)) != FG_OK) return st;
-  const int grid = min(kAttnMaxGrid, dev.sm_count * attn_ctas_per_sm(cols));
+  const int grid = min(kAttnMaxGrid, dev.sm_count * kAttnCtasPerSm);
   return host::launch(kern, dim3(grid), dim3(kAttnThreads), smem, reinterpret_cast<cudaStream_t>(stream), true, p);
 }

@@ -210,6 +210,20 @@ def test_ranges_of_keys_and_values(spread, offset, dev):
     _check_attention(_attend(pool, table, q, lens, 16, starts, dev, scale), pool, table, q, lens, 16, starts, scale)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_long_sums_keep_their_precision(d, dev):
+    """Averages of thousands of values are small beside them: what sums of one sign lose on the way shows here.  Rounded once,
+    exact outputs are at most half a step off each, in the mean 0.4 of that; so half a step bounds the error of all of them
+    (weights of eleven bits alone make it 2^-11 * 2.7 / 2.4, sums that are cut off at every product 2^-11 * 3.3 / 2.4)."""
+    n, page = 8000, 16
+    pool, table, q, _ = _case([n], None, 8, 8, d, page, 71)
+    lens = [n] * 40
+    table, q = table.repeat(40, 1), torch.randn(40, 8, d, generator=torch.Generator().manual_seed(72)).half()
+    out = _attend(pool, table, q, lens, page, None, dev).cpu().to(torch.float64)
+    want, _, _ = ref.attention(q, pool, table, lens, page)
+    assert float((out - want).norm()) <= 2.0 ** -11 * float(want.norm())
+
+
 def test_constant_values_and_rising_scores(dev):
     """Rows whose values are all alike (the smallest scale) beside ordinary ones, and scores that rise along the sequence, so
     that the running maximum moves again and again."""
