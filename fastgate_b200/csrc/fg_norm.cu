@@ -7,7 +7,9 @@
 // One pass: a row stays in its CTA's registers between the load and the store, and both statistics (sum of
 // squares and largest |t|) go through one block reduction.  The int8 codes are formed from t, not from the
 // normalised value: rstd divides out of y / scale, so the reduction's summation order cannot move a code.
-// The traffic is the bound: 2 K bytes of x, 4 K (8 K) of residual in and out in fp16 (fp32), 2 K or K of output.
+// The traffic is the bound: 2 K bytes of x, 4 K (8 K) of residual in and out in fp16 (fp32), 2 K or K of output.  Measured on
+// B200, int8 output: 8192 x 4096 with an fp32 residual 56.3 us (6.6 TB/s, a plain copy's rate), with an fp16 one 40.9 (5.8 TB/s); 16 x
+// 8192 2.4 us, of which a launch is most.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -209,11 +211,13 @@ extern "C" int fg_add_rmsnorm(const void* x, long long ldx, const void* weight, 
   host::Device dev;
   const int st = host::current_device(&dev);
   if (st != FG_OK) return st;
-  // Few rows: as many threads a row as it has vectors, the latency of one load is all there is.  Many rows: four
-  // vectors a thread, so that fewer threads meet in each reduction and each has more loads in flight.
-  const int nvec = K / 8;
-  int vpt = M <= 2 * dev.sm_count ? 1 : 4;
-  while (vpt < 4 && (nvec + vpt - 1) / vpt > kNormMaxThreads) vpt *= 2;
+  // Few rows: as many threads a row as it has vectors, the latency of one load is all there is (16 x 8192 2.4 us, with 512
+  // threads 2.8; 296 x 8192 3.7 / 4.1).  Many rows: 512 threads at most, whose CTAs do not leave an SM half empty between two
+  // rows (4096 x 8192, fp16 residual: 42.2 us with 512 threads, 44.5 with 1024; 2048 x 16384: 49.6 / 55.1; fewer threads with
+  // more vectors each are slower too: 8192 x 4096 40.9 with 512, 44.5 with 128).
+  const int nvec = K / 8, most_threads = M <= 2 * dev.sm_count ? kNormMaxThreads : kNormMaxThreads / 2;
+  int vpt = 1;
+  while (vpt < 4 && (nvec + vpt - 1) / vpt > most_threads) vpt *= 2;
   int threads = ((nvec + vpt - 1) / vpt + 31) / 32 * 32;
   if (threads > kNormMaxThreads) {
     vpt = 0;
