@@ -73,7 +73,8 @@ __host__ __device__ constexpr int attn_smem_bytes(int d, int cols) { return kAtt
 // 8000 rows 95 / 99 us, one of 5000 11.1 / 13.7.  A third ring slot changes neither.  Sixteen columns, 24 x 3000 rows of 64
 // channels, two / three / four CTAs: 20.6 / 22.9 / 28.4, before the second operand of the weights.)
 constexpr int kAttnCtasPerSm = 2;
-constexpr int kAttnMaxCols = 16;
+constexpr int kAttnMostFloats = partial_floats(64, 16);  // of a partial; eight columns of 128 channels take less
+static_assert(partial_floats(128, 8) <= kAttnMostFloats, "workspace");
 
 struct AttnParams {
   const __half* q;        // [tokens, q_heads, D], token stride ldq
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) fg_kv_attention_
   constexpr int kSet = 32 / kSlotBlocks;  // slots whose blocks the lanes of a warp hold
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) unsigned long long bars[kAttnWarps * S];
-  __shared__ uint32_t scan[kAttnWarps], start_before;
+  __shared__ uint32_t scan[kAttnWarps], scan_rough[kAttnWarps], start_before;
   __shared__ int start_b;
   __shared__ Pending pending[2];
   __shared__ float warp_max[kAttnWarps][COLS], warp_norm[kAttnWarps][COLS];
@@ -225,21 +226,31 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) fg_kv_attention_
   const int kv_heads = p.kv.heads;
   const int per = (p.batch + kAttnThreads - 1) / kAttnThreads;
   const int b_lo = min(p.batch, tid * per), b_hi = min(p.batch, b_lo + per);
-  uint32_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += sequence<COLS>(p, b, blockIdx.x == 0).total(kv_heads);
+  unsigned long long sum = 0;
+  for (int b = b_lo; b < b_hi; ++b) sum += sequence<COLS>(p, b, blockIdx.x == 0).total(kv_heads);
+  const uint32_t mine = static_cast<uint32_t>(min(sum, 0x80000000ull));
   uint32_t incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const uint32_t v = __shfl_up_sync(0xffffffffu, incl, off);
     if (lane >= off) incl += v;
   }
-  if (lane == 31) scan[warp] = incl;
+  const uint32_t rough = __reduce_add_sync(0xffffffffu, mine >> 12);
+  if (lane == 31) {
+    scan[warp] = incl;
+    scan_rough[warp] = rough;
+  }
   __syncthreads();
-  uint32_t before = incl - mine, total = 0;
+  uint32_t before = incl - mine, total = 0, all_rough = 0;
 #pragma unroll
   for (int w = 0; w < kAttnWarps; ++w) {
     if (w < warp) before += scan[w];
     total += scan[w];
+    all_rough += scan_rough[w];
+  }
+  if (all_rough >= 0x80000u - kAttnThreads) {  // about 2^31 units, more than q has rows for: q_starts overlap
+    if (tid == 0 && blockIdx.x == 0 && p.status != nullptr) atomicExch(p.status, kStatusIndex);
+    return;
   }
   const uint32_t chunk = (total + gridDim.x - 1) / gridDim.x;
   const uint32_t cta = blockIdx.x, ub = cta * chunk, ue = min(total, ub + chunk);
@@ -291,7 +302,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) fg_kv_attention_
     const int i = kSet * set + lane / kSlotBlocks, blk = (c_first + i * kAttnWarps) * kSlotBlocks + lane % kSlotBlocks;
     at = kNoBlock;
     if (i < c_slots && blk * kKvBlock < cw.sq.len) {
-      const int nth = blk / blocks_per_page, page = __ldg(p.table + static_cast<long long>(cw.b) * p.ldt + nth);
+      const int nth = blk / blocks_per_page, page = p.table[static_cast<long long>(cw.b) * p.ldt + nth];
       if (page >= 0 && page < p.kv.pages)
         at = (static_cast<uint32_t>(page) * kv_heads + c_head) * blocks_per_page + (blk - nth * blocks_per_page);
       else if (p.status != nullptr)
@@ -779,7 +790,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) fg_kv_attention_
 }  // namespace fg
 
 extern "C" size_t fg_kv_attention_workspace_bytes(void) {
-  return fg::kAttnPartialsOffset + static_cast<size_t>(fg::kAttnMaxGrid) * 2 * fg::partial_floats(128, fg::kAttnMaxCols) * sizeof(float);
+  return fg::kAttnPartialsOffset + static_cast<size_t>(fg::kAttnMaxGrid) * 2 * fg::kAttnMostFloats * sizeof(float);
 }
 
 extern "C" int fg_kv_attention_workspace_init(void* ws, size_t ws_bytes, fg_stream_t stream) {
@@ -803,7 +814,7 @@ extern "C" int fg_kv_attention_int4(const void* q, long long ldq, void* out, lon
   // work units and block numbers are 32-bit in the kernel; an upper bound of both, whatever the lengths turn out to be
   const long long group = q_heads / kv_heads;
   const double most_units = (static_cast<double>(tokens) * group / 8 + batch) * kv_heads * (static_cast<double>(table_width) * page_size / kUnitRows + 1);
-  if (most_units >= 2147483648.0 || static_cast<double>(num_pages) * kv_heads * (page_size / kKvBlock) >= 4294967295.0) return FG_ERR_SHAPE;
+  if (most_units >= 2146900000.0 || static_cast<double>(num_pages) * kv_heads * (page_size / kKvBlock) >= 4294967295.0) return FG_ERR_SHAPE;
   if (!host::aligned(q, 16) || !host::aligned(out, 16) || !host::aligned(pages, 16) || !host::aligned(block_table, 4) ||
       !host::aligned(seq_lens, 4) || !host::aligned(q_starts, 4) || !host::aligned(status_dev, 4))
     return FG_ERR_ALIGN;
@@ -830,13 +841,14 @@ extern "C" int fg_kv_attention_int4(const void* q, long long ldq, void* out, lon
   p.tickets = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(ws) + kAttnTicketsOffset);
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kAttnPartialsOffset);
   p.status = status_dev;
-  // Eight columns where a sequence's queries of one key/value head fit them, else sixteen.  (Thirty-two, for 64 channels, leave
-  // eight warps on an SM: 33.7 us against 23.1 on 24 x 3000 rows with up to 40 columns a sequence.)
+  // Sixteen columns where a sequence has more than eight queries of a key/value head and a head 64 channels: half the unpacking
+  // (24 x 3000 rows, 16 columns a sequence: 24.7 us, with eight 29.2; 48 columns: 39.2 / 43.5; thirty-two columns leave too
+  // few registers).  With 128 channels the registers spill and eight are as good or better (16 columns 38.1 / 38.6, 48 columns
+  // 61.3 / 60.0, 64 x 500 rows 62.1 / 56.1).
   const long long per_seq = (tokens + batch - 1) / batch * p.group;
-  int cols = 8;
-  if (per_seq > cols) cols = kAttnMaxCols;
-  void (*kern)(const AttnParams) = d == 128 ? (cols == 16 ? fg_kv_attention_kernel<128, 2> : fg_kv_attention_kernel<128, 1>)
-                                   : (cols == 16 ? fg_kv_attention_kernel<64, 2> : fg_kv_attention_kernel<64, 1>);
+  const int cols = d == 64 && per_seq > 8 ? 16 : 8;
+  void (*kern)(const AttnParams) =
+      d == 128 ? fg_kv_attention_kernel<128, 1> : cols == 16 ? fg_kv_attention_kernel<64, 2> : fg_kv_attention_kernel<64, 1>;
   const int smem = attn_smem_bytes(d, cols);
   if ((st = host::opt_in_smem(reinterpret_cast<const void*>(kern), smem)) != FG_OK) return st;
   const int grid = min(kAttnMaxGrid, dev.sm_count * kAttnCtasPerSm);

@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kGemv8Warps * 32) fg_gemv8_kernel(const Gemv8P
       if (at + 32 * i < pieces) {
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-          const uint4 v = __ldg(x + static_cast<size_t>(m) * pieces + at + 32 * i);
+          const uint4 v = x[static_cast<size_t>(m) * pieces + at + 32 * i];
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             acc[r][m] = __dp4a(static_cast<int>(q[i][r].x), static_cast<int>(v.x), acc[r][m]);

@@ -114,9 +114,8 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
     const float* t = p.cos_sin + pos * D;
     // pairs (i, i + D/2): angles 8 lane..; pairs (2i, 2i + 1): angles 4 lane.. of the lower and of the upper half
     const int a0 = p.interleaved ? 4 * lane : 8 * lane, a1 = p.interleaved ? D / 4 + 4 * lane : 8 * lane + 4;
-    const float4 c0 = __ldg(reinterpret_cast<const float4*>(t + a0)), c1 = __ldg(reinterpret_cast<const float4*>(t + a1));
-    const float4 s0 = __ldg(reinterpret_cast<const float4*>(t + D / 2 + a0));
-    const float4 s1 = __ldg(reinterpret_cast<const float4*>(t + D / 2 + a1));
+    const float4 c0 = *reinterpret_cast<const float4*>(t + a0), c1 = *reinterpret_cast<const float4*>(t + a1);
+    const float4 s0 = *reinterpret_cast<const float4*>(t + D / 2 + a0), s1 = *reinterpret_cast<const float4*>(t + D / 2 + a1);
     cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w; cs[4] = c1.x; cs[5] = c1.y; cs[6] = c1.z; cs[7] = c1.w;
     sn[0] = s0.x; sn[1] = s0.y; sn[2] = s0.z; sn[3] = s0.w; sn[4] = s1.x; sn[5] = s1.y; sn[6] = s1.z; sn[7] = s1.w;
   } else {
@@ -213,8 +212,7 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_read_kernel(const ReadParams
   const int lane = threadIdx.x % LPR;
   const long long token = static_cast<long long>(blockIdx.x) * (kKvThreads / LPR) + threadIdx.x / LPR;
   const int head0 = blockIdx.y * HPT;
-  griddep_launch_dependents();
-  griddep_wait();
+  griddep_wait();  // (no early launch of the next kernel: these rows may be what a linear takes for its weight, which it reads at once)
   if (token >= p.tokens) return;
   const long long slot = p.slots[token];
   if (slot < 0) return;

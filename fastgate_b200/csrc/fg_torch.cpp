@@ -244,8 +244,12 @@ int64_t workspace_status(int64_t device) {
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
   const Workspace ws = workspace_for(static_cast<int>(device), stream, 128);
   int v = -1;
-  const int st = fg_workspace_status(ws.buf.data_ptr(), &v, reinterpret_cast<fg_stream_t>(stream));
+  int st = fg_workspace_status(ws.buf.data_ptr(), &v, reinterpret_cast<fg_stream_t>(stream));
   if (st != FG_OK) raise(st, true);
+  if (v == FG_OK) {
+    st = fg_workspace_status(linear_status(static_cast<int>(device)), &v, reinterpret_cast<fg_stream_t>(stream));
+    if (st != FG_OK) raise(st, true);
+  }
   return v;
 }
 
@@ -408,18 +412,6 @@ void hgemm_tr(at::Tensor A, at::Tensor W, at::Tensor C) {
 }
 
 }  // namespace
-
-int* linear_status(int64_t device, cudaStream_t stream) {
-  {
-    // (a captured call only borrows what is there: the workspace's first use clears it, which is no work for a graph)
-    std::lock_guard<std::mutex> lk(g_ws_mu);
-    const auto w = g_ws.find({static_cast<int>(device), reinterpret_cast<int64_t>(stream)});
-    if (w != g_ws.end() && w->second.bytes > 0) return static_cast<int*>(w->second.buf.data_ptr());
-  }
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) return nullptr;
-  return static_cast<int*>(workspace_for(static_cast<int>(device), stream, 128).buf.data_ptr());
-}
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "fastgate_b200: B200 (sm_100a) small-batch matmul operators with the SPEEDGATE surface";

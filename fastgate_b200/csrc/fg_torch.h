@@ -5,9 +5,9 @@
 
 // The cleared workspace of a call that is being captured on `stream` (fg_torch_graph.cpp); nullptr: no capture.
 void* graph_workspace(int device, cudaStream_t stream, size_t bytes);
-// The status word that workspace_status() reads: of the stream's workspace (fg_torch.cpp).  nullptr while the stream is
-// captured and has none yet.
-int* linear_status(int64_t device, cudaStream_t stream);
+// The device's status word of the operators that have no workspace (fg_torch_graph.cpp): allocated once and kept, so that
+// captured calls may hold it.  workspace_status() reads it too.
+int* linear_status(int device);
 
 // Operators around the linears of a serving step (fg_torch_serving.cpp).
 void bind_serving(pybind11::module& m);

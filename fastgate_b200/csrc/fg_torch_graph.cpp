@@ -66,7 +66,34 @@ struct RelaxedMode {
   ~RelaxedMode() { cudaThreadExchangeStreamCaptureMode(&mode); }
 };
 
+// On a stream of its own, to the end.
+void clear(void* p, size_t bytes) {
+  cudaStream_t side = nullptr;
+  must(cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking));
+  cudaError_t e = cudaMemsetAsync(p, 0, bytes, side);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(side);
+  cudaStreamDestroy(side);
+  must(e);
+}
+
+// `bytes` of zeros on the current device, also while a stream is being captured.
+void* cleared(size_t bytes) {
+  RelaxedMode relaxed;
+  void* p = nullptr;
+  must(cudaMalloc(&p, bytes));
+  clear(p, bytes);
+  return p;
+}
+
 }  // namespace
+
+int* linear_status(int device) {
+  static std::map<int, void*>* words = new std::map<int, void*>;
+  std::lock_guard<std::mutex> lk(mu());
+  void*& p = (*words)[device];
+  if (p == nullptr) p = cleared(256);
+  return static_cast<int*>(p);
+}
 
 void* graph_workspace(int device, cudaStream_t stream, size_t bytes) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
@@ -89,15 +116,10 @@ void* graph_workspace(int device, cudaStream_t stream, size_t bytes) {
     blocks().push_back(b);
   }
   Block& b = blocks()[index];
-  cudaStream_t side = nullptr;
-  must(cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking));
-  cudaError_t e = cudaMemsetAsync(b.ptr, 0, b.bytes, side);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(side);
-  cudaStreamDestroy(side);
-  must(e);
+  clear(b.ptr, b.bytes);
   Release* r = new Release{index, key};
   cudaUserObject_t object = nullptr;
-  e = cudaUserObjectCreate(&object, r, release, 1, cudaUserObjectNoDestructorSync);
+  cudaError_t e = cudaUserObjectCreate(&object, r, release, 1, cudaUserObjectNoDestructorSync);
   if (e != cudaSuccess) {
     delete r;
     must(e);

@@ -92,6 +92,9 @@ void add_rmsnorm(at::Tensor x, at::Tensor weight, at::Tensor out, OptTensor resi
   if (int8) {
     check_dense(*scales, "scales", at::kFloat, device);
     if (scales->numel() != M) bad_argument("scales must hold one fp32 value per row");
+    if (overlap(*scales, x) || overlap(*scales, out) || overlap(*scales, weight) || (given(residual) && overlap(*scales, *residual)) ||
+        (given(residual_out) && overlap(*scales, *residual_out)))
+      bad_argument("scales must not overlap the other buffers");
   }
   const void* res = nullptr;
   void* res_out = nullptr;
@@ -171,7 +174,7 @@ void linear_int8(at::Tensor x8, at::Tensor W8, at::Tensor C, at::Tensor x_scales
     bad_argument("the output may be the residual itself; otherwise it must not overlap the inputs");
   const c10::cuda::CUDAGuard guard(x8.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(device).stream();
-  int* status = linear_status(device, stream);
+  int* status = linear_status(static_cast<int>(device));
   int st;
   {
     pybind11::gil_scoped_release nogil;
@@ -257,7 +260,7 @@ void kv_read_int4(at::Tensor pages, at::Tensor slots, at::Tensor k_out, at::Tens
   check_pages(pages, page_size, heads, d, device);
   const int slots64 = check_index(slots, "slots", T, device);
   int* sp = status_ptr(status, device);
-  if (overlap(k_out, v_out)) bad_argument("k_out and v_out must not overlap");
+  if (overlap(k_out, v_out) || overlap(k_out, pages) || overlap(v_out, pages)) bad_argument("k_out, v_out and pages must not overlap");
   if (T == 0 || heads == 0) return;
   if (heads > 16384) bad_argument("too many heads");
   const c10::cuda::CUDAGuard guard(k_out.device());

@@ -290,6 +290,40 @@ def test_bad_indices_are_reported(dev):
     assert torch.equal(pool_out, good)
 
 
+def test_overlapping_query_ranges_are_refused_before_they_overflow(dev):
+    """q_starts that go back and forth give every other sequence all of q: more work units than 32 bits count."""
+    tokens, batch, page = 16384, 64, 128
+    q = torch.zeros(tokens, 64, 64, dtype=torch.half, device=dev)
+    out = torch.full_like(q, 3.0)
+    pool = torch.zeros(2, 8, page * 72, dtype=torch.uint8, device=dev)
+    table = torch.zeros(1, 2048, dtype=torch.int32, device=dev).expand(batch, -1).contiguous()
+    lens = torch.full((batch,), 2048 * page, dtype=torch.int32, device=dev)
+    starts = torch.tensor([0, tokens] * (batch // 2) + [0], dtype=torch.int32, device=dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    fg.kv_attention_int4(q, pool, table, lens, out, page, starts, None, status)
+    assert int(status) == capi.FG_ERR_INDEX and bool((out == 3.0).all())
+
+
+def test_rows_read_back_may_be_the_weight_of_the_next_call(dev):
+    """A linear asks for its weight while the kernel before it still runs; rows that kv_read_int4 has just written are whole."""
+    n, d, page = 4096, 128, 64
+    pool = ref.random_pages(torch.Generator().manual_seed(3), n // page, 1, d, page).to(dev)
+    slots = torch.arange(n, device=dev)
+    x = torch.randn(16, d, generator=torch.Generator().manual_seed(4)).half().to(dev)
+    k, v = (torch.empty(n, 1, d, dtype=torch.half, device=dev) for _ in range(2))
+    c = torch.empty(16, n, dtype=torch.half, device=dev)
+    fg.kv_read_int4(pool, slots, k, v, page)
+    torch.cuda.synchronize()
+    fg.edgemm_m8n128k64x4_bt(x, k.view(n, d), c)
+    want = c.clone()
+    torch.cuda.synchronize()
+    for _ in range(50):
+        k.zero_()
+        fg.kv_read_int4(pool, slots, k, v, page)
+        fg.edgemm_m8n128k64x4_bt(x, k.view(n, d), c)
+        assert torch.equal(c, want)
+
+
 def test_strides_and_scale(dev):
     """Queries out of a fused projection, output into a wider buffer, a table with a row stride."""
     lens, page = [70, 33, 90], 16

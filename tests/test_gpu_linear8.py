@@ -209,3 +209,18 @@ def test_refusals(dev):
     args = lambda act=0, xs=s.data_ptr(): capi.lib.fg_linear_w8a8(x.data_ptr(), w.data_ptr(), xs, 1, None, c.data_ptr(), 2, 128, 256, None, None, act,
                                                                   None, ctypes.c_void_p(0))
     assert args(act=9) == capi.FG_ERR_PLAN and args(xs=None) == capi.FG_ERR_NULL
+
+
+def test_captured_before_any_eager_call(dev):
+    """A stream's first call may be a captured one; the status word that it holds is the one that workspace_status() reads."""
+    x8, w8, xs, ws, *_ = _data(9, 256, 512, 77)
+    a = [t.to(dev) for t in (x8, w8, xs, ws)]
+    c = torch.empty(9, 256, dtype=torch.half, device=dev)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        fg.linear_int8(a[0], a[1], c, a[2], a[3])
+    for _ in range(3):
+        graph.replay()
+    want = torch.empty_like(c)
+    fg.linear_int8(a[0], a[1], want, a[2], a[3])
+    assert torch.equal(c, want) and fg.workspace_status(0) == 0
