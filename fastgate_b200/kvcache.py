@@ -46,9 +46,14 @@ class KVCacheInt4:
 
     def slots(self, block_table: torch.Tensor, sequence: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Slot of each row: page block_table[sequence, position // page_size], row position % page_size.  A negative
-        position (a padding row) gets slot -1."""
-        at = positions.long().clamp(min=0)
-        slot = block_table[sequence.long(), at // self.page_size].long() * self.page_size + at % self.page_size
+        position (a padding row) gets slot -1; a row that the table has no page for, the slot behind the last one, which
+        append and read leave out and check() reports."""
+        rows, width = block_table.shape
+        seq, at = sequence.long(), positions.long().clamp(min=0)
+        nth = at // self.page_size
+        page = block_table[seq.clamp(0, rows - 1), nth.clamp(max=width - 1)].long()
+        known = (seq >= 0) & (seq < rows) & (nth < width) & (page >= 0)
+        slot = torch.where(known, page * self.page_size + at % self.page_size, self.pages.shape[0] * self.page_size)
         return torch.where(positions >= 0, slot, -1)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cos_sin: Optional[torch.Tensor] = None,

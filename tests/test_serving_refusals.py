@@ -97,6 +97,14 @@ def test_rotation_table_keeps_far_angles():
     assert float((t[200000].double() - torch.cat([a.cos(), a.sin()])).abs().max()) <= 2.0 ** -24
 
 
+def test_slots_of_rows_without_a_page():
+    """No page in the table, no such column, no such sequence: the slot behind the pool, which the kernels report."""
+    cache = KVCacheInt4(8, 2, 64, page_size=32, device="cpu")
+    table = torch.tensor([[3, -1], [5, 1]], dtype=torch.int32)
+    got = cache.slots(table, torch.tensor([0, 0, 1, 1, 2, -1, 1]), torch.tensor([0, 40, 63, 64, 0, 0, -5]))
+    assert got.tolist() == [96, 256, 63, 256, 256, 256, -1]
+
+
 def test_tilings_of_the_linear_are_launchable():
     """Every choice: a known tile, a cluster only where its tiles fit the card at once, no CTA without a stage of k, the
     followers' sums within the leader's ring."""
