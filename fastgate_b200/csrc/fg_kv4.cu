@@ -6,8 +6,8 @@
 // format has.  2^-24 is the smallest positive fp16: a constant row gets it instead of a division by zero.
 //
 // Both kernels move each byte once.  Measured on B200: read 40000 rows of 8 heads of 128 channels 38.6 us (5.4 TB/s, nine
-// tenths of it stores), append 6001 tokens of 48 heads of 64 channels 17.7 us (3.8 TB/s: each lane waits for its slot, then for
-// its rows; issue slots are half full), and 64 tokens 2.6, 500 rows read 1.9 us, which is a launch and those latencies.
+// tenths of it stores), append 6001 tokens of 48 heads of 64 channels 17.1 us (3.9 TB/s: each lane waits for its slot, then for
+// its rows; issue slots are half full), and 64 tokens 2.3, 500 rows read 1.9 us, which is a launch and those latencies.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -87,21 +87,20 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
   griddep_wait();
 
   // A padding token (negative slot) is left out whole; an index out of range too, and reported.
-  const long long slot = token < p.tokens ? p.slots[token] : -1;
-  bool go = slot >= 0 && slot < p.kv.pages * p.kv.page_size;
-  long long pos = 0;
-  if (go && p.cos_sin != nullptr) {
-    pos = p.positions[token];
-    go = pos >= 0 && pos < p.positions_len;
-  }
+  const bool there = token < p.tokens;
+  const long long slot = there ? p.slots[token] : -1;
+  const long long pos = there && p.cos_sin != nullptr ? p.positions[token] : 0;
+  const bool placed = p.cos_sin == nullptr || (pos >= 0 && pos < p.positions_len);
+  const bool go = slot >= 0 && slot < p.kv.pages * p.kv.page_size && placed;
   if (slot >= 0 && !go && lane == 0 && p.status != nullptr) atomicExch(p.status, kStatusIndex);
-
   uint4 raw[HPT][2];
 #pragma unroll
   for (int i = 0; i < HPT; ++i) {
     const int h = head0 + i;
     raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
-    if (go && h < heads) {
+    // One head: the row is asked for without waiting for its slot, also a padding token's (64 tokens: 2.3 us, else 2.5).  Four
+    // heads: after the slot (6001 tokens of 48 heads: 17.1 us, else 19.2).
+    if ((HPT == 1 ? there : go) && h < heads) {
       const __half* src = h < p.q_heads ? p.q + token * p.ldq + static_cast<long long>(h) * D
                           : h < turned  ? p.k + token * p.ldk + static_cast<long long>(h - p.q_heads) * D
                                         : p.v + token * p.ldv + static_cast<long long>(h - turned) * D;
@@ -111,7 +110,7 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
   }
   const bool rotate = p.cos_sin != nullptr && head0 < turned;
   float cs[8], sn[8];
-  if (rotate && go) {
+  if (rotate && there && placed) {
     const float* t = p.cos_sin + pos * D;
     // pairs (i, i + D/2): angles 8 lane..; pairs (2i, 2i + 1): angles 4 lane.. of the lower and of the upper half
     const int a0 = p.interleaved ? 4 * lane : 8 * lane, a1 = p.interleaved ? D / 4 + 4 * lane : 8 * lane + 4;
@@ -161,7 +160,7 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
       }
       continue;
     }
-    // every lane of the warp takes part in the row reductions; rows that store nothing reduce zeros
+    // every lane of the warp takes part in the row reductions; rows that store nothing are reduced too
     float mn = fminf(lo[0], hi[0]), mx = fmaxf(lo[0], hi[0]), bad = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -306,7 +305,7 @@ extern "C" int fg_kv_append_int4(const void* k, long long ldk, const void* v, lo
   p.status = status_dev;
   p.tokens = tokens;
   // Few rows: one a lane group, for latency; enough rows for two CTAs' worth a SM with four: four (6001 tokens of 48 heads of
-  // 64 channels: 17.7 us against 19.9).
+  // 64 channels: 17.1 us, with one 21.6; 64 tokens: 2.3 us, with four 4.7).
   const long long heads = q_heads + 2LL * kv_heads, rows_per_cta = kKvThreads / (d / 16);
   const bool many = tokens * heads >= 4 * 4 * rows_per_cta * dev.sm_count;
   const long long gx = (tokens + rows_per_cta - 1) / rows_per_cta, gy = (heads + (many ? 3 : 0)) / (many ? 4 : 1);
