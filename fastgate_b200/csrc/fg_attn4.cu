@@ -9,7 +9,7 @@
 // The bytes of the cache are the floor: D + 8 of them per row and head, against 16 D bit operations' worth of
 // unpacking.  Measured on B200 (64 / 8 heads of 128 channels): 64 sequences of up to 8000 rows 93.6 us, 4.2 TB/s, with the tensor pipe
 // 38 % and the integer pipe 43 % busy: the latency of dependent instructions at two warps a scheduler bounds it.  One sequence of
-// 5000 rows (32 / 8 heads) 11.2 us: lengths, table, rows, partial sums, ticket, join, each a trip to L2 or memory.
+// 5000 rows (32 / 8 heads) 10.4 us: lengths, table, rows, partial sums, ticket, join, each a trip to L2 or memory.
 // What this kernel does about the unpacking:
 //   - A code's four bits, masked in place, ARE an fp16 number: bits 0-3 of a half are the subnormal code * 2^-24, bits 4-7
 //     code * 2^-20.  The tensor core multiplies subnormals exactly, so unpacking is one AND per two codes (and one shift
@@ -362,7 +362,6 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) fg_kv_attention_
   };
   // Output: a thread has four channels of every (kAttnThreads / (D / 4))th column.
   constexpr int TPC = D / 4;
-  constexpr uint32_t kJoin = 8;
   const int d4 = (tid % TPC) * 4;
   auto write_out = [&](int flat, int head, int q0, float4 v, float l) {
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
@@ -728,59 +727,72 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) fg_kv_attention_
     if (q.ticket != q.parts - 1) continue;
     const float* first = p.partials + static_cast<size_t>(q.first * 2) * partial_floats(D, COLS);
     auto part_of = [&](uint32_t x) { return first + static_cast<size_t>(2 * x + (x == 0 ? q.first_slot : 0)) * partial_floats(D, COLS); };
-    // With L2 most of a microsecond away it is the number of dependent passes that counts: two columns of a thread and kJoin
-    // partials of each are asked for at once, the maxima among them.
+    // With L2 most of a microsecond away it is the number of dependent passes that counts: a thread asks for 24 partials of its
+    // column at once, maxima included, or for 8 of each of two columns where there are more than one per thread (one sequence of
+    // 5000 rows in 20 parts: 10.4 us, with 8 at once 11.2).
     constexpr int kStep = kAttnThreads / TPC;
+    auto join = [&](auto columns) {
+      constexpr int Y = decltype(columns)::value;
+      constexpr uint32_t kParts = Y == 1 ? 24 : 8;
 #pragma unroll 1
-    for (int col0 = tid / TPC; col0 < q.cols; col0 += 2 * kStep) {
-      float m[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
-      float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+      for (int col0 = tid / TPC; col0 < q.cols; col0 += Y * kStep) {
+        float m[Y], l[Y];
+        float4 v[Y];
+#pragma unroll
+        for (int y = 0; y < Y; ++y) {
+          m[y] = kNoMax;
+          l[y] = 0.f;
+          v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
 #pragma unroll 1
-      for (uint32_t x0 = 0; x0 < q.parts; x0 += kJoin) {
-        float4 a[kJoin][2];
-        float mx[kJoin][2], lx[kJoin][2];
+        for (uint32_t x0 = 0; x0 < q.parts; x0 += kParts) {
+          float4 a[kParts][Y];
+          float mx[kParts][Y], lx[kParts][Y];
 #pragma unroll
-        for (uint32_t i = 0; i < kJoin; ++i)
+          for (uint32_t i = 0; i < kParts; ++i)
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-            if (x0 + i < q.parts && col0 + y * kStep < q.cols) {
-              const float* src = part_of(x0 + i);
-              const int col = col0 + y * kStep;
-              a[i][y] = __ldcg(reinterpret_cast<const float4*>(src + col * D + d4));
-              mx[i][y] = __ldcg(src + COLS * D + col);
-              lx[i][y] = __ldcg(src + COLS * D + COLS + col);
-            } else {
-              a[i][y] = make_float4(0.f, 0.f, 0.f, 0.f);
-              mx[i][y] = kNoMax;
-              lx[i][y] = 0.f;
+            for (int y = 0; y < Y; ++y)
+              if (x0 + i < q.parts && col0 + y * kStep < q.cols) {
+                const float* src = part_of(x0 + i);
+                const int col = col0 + y * kStep;
+                a[i][y] = __ldcg(reinterpret_cast<const float4*>(src + col * D + d4));
+                mx[i][y] = __ldcg(src + COLS * D + col);
+                lx[i][y] = __ldcg(src + COLS * D + COLS + col);
+              } else {
+                a[i][y] = make_float4(0.f, 0.f, 0.f, 0.f);
+                mx[i][y] = kNoMax;
+                lx[i][y] = 0.f;
+              }
+#pragma unroll
+          for (int y = 0; y < Y; ++y) {
+            float top = m[y];
+#pragma unroll
+            for (uint32_t i = 0; i < kParts; ++i) top = fmaxf(top, mx[i][y]);
+            const float back = ex2(m[y] - top);
+            m[y] = top;
+            l[y] *= back;
+            v[y].x *= back;
+            v[y].y *= back;
+            v[y].z *= back;
+            v[y].w *= back;
+#pragma unroll
+            for (uint32_t i = 0; i < kParts; ++i) {
+              const float f = ex2(mx[i][y] - top);
+              l[y] = fmaf(f, lx[i][y], l[y]);
+              v[y].x = fmaf(f, a[i][y].x, v[y].x);
+              v[y].y = fmaf(f, a[i][y].y, v[y].y);
+              v[y].z = fmaf(f, a[i][y].z, v[y].z);
+              v[y].w = fmaf(f, a[i][y].w, v[y].w);
             }
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          float top = m[y];
-#pragma unroll
-          for (uint32_t i = 0; i < kJoin; ++i) top = fmaxf(top, mx[i][y]);
-          const float back = ex2(m[y] - top);
-          m[y] = top;
-          l[y] *= back;
-          v[y].x *= back;
-          v[y].y *= back;
-          v[y].z *= back;
-          v[y].w *= back;
-#pragma unroll
-          for (uint32_t i = 0; i < kJoin; ++i) {
-            const float f = ex2(mx[i][y] - top);
-            l[y] = fmaf(f, lx[i][y], l[y]);
-            v[y].x = fmaf(f, a[i][y].x, v[y].x);
-            v[y].y = fmaf(f, a[i][y].y, v[y].y);
-            v[y].z = fmaf(f, a[i][y].z, v[y].z);
-            v[y].w = fmaf(f, a[i][y].w, v[y].w);
           }
         }
-      }
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
-        if (col0 + y * kStep < q.cols) write_out(q.tile * COLS + col0 + y * kStep, q.head, q.q0, v[y], l[y]);
-    }
+        for (int y = 0; y < Y; ++y)
+          if (col0 + y * kStep < q.cols) write_out(q.tile * COLS + col0 + y * kStep, q.head, q.q0, v[y], l[y]);
+      }
+    };
+    if (q.cols <= kStep) join(std::integral_constant<int, 1>{});
+    else join(std::integral_constant<int, 2>{});
     if (tid == 0) p.tickets[q.first] = 0;  // ready for the next launch
   }
   if (dead) {
