@@ -4,6 +4,10 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <array>
+#include <map>
+#include <mutex>
+
 #include "../../include/fastgate_b200.h"
 #include "fg_gemm8.cuh"
 #include "fg_gemv8.cuh"
@@ -51,7 +55,8 @@ int stages_of(const TileCost& c, int smem_optin) {
 
 // The tiling with the least estimated time: per wave of tiles its blocks of k or its share of the bytes, whichever takes
 // longer (a last wave of a few tiles costs as much as a full one where the tensor cores bound it, little where memory does).
-Tiling choose_tiling(int M, int N, int K, bool gated, int sm_count, int smem_optin) {
+// clusters: how many clusters of 2, 4 and 8 CTAs the device holds at once.
+Tiling choose_tiling(int M, int N, int K, bool gated, int sm_count, int smem_optin, const int (&clusters)[3]) {
   const double dram = (static_cast<double>(N) * K + static_cast<double>(M) * K + 2.0 * M * N) / kDramBytesPerUs;
   Tiling best = {128, 1, 1};
   double best_us = 1e30;
@@ -60,10 +65,10 @@ Tiling choose_tiling(int M, int N, int K, bool gated, int sm_count, int smem_opt
     const long long tiles = static_cast<long long>((M + 128 * c.cg - 1) / (128 * c.cg)) * ((N + c.bn - 1) / c.bn);
     const int per = fg::gemm8_blocks_per_stage(c.cg, c.bn), k_stages = (K / 128 + per - 1) / per;
     const int ring = stages_of(c, smem_optin) * fg::gemm8_stage_bytes(c.cg, c.bn);
-    for (int s = 1; s <= (c.cg == 1 ? 8 : 1); s *= 2) {
-      // A cluster lives in one GPC: up to seven eighths of the SMs can be counted on.  Every CTA has a stage at least, and the
-      // followers' sums fit in the leader's ring.
-      if (s > 1 && (tiles * s > sm_count - sm_count / 8 || k_stages < s || (s - 1) * c.bn * 512 > ring)) break;
+    for (int s = 1, log = 0; s <= (c.cg == 1 ? 8 : 1); s *= 2, ++log) {
+      // All clusters run at once (a second wave of a few costs as much again: 16 x 512 x 8192 15.6 us with 16 clusters of 8 on a
+      // device that holds fewer).  Every CTA has a stage at least, and the followers' sums fit in the leader's ring.
+      if (s > 1 && (tiles > clusters[log - 1] || k_stages < s || (s - 1) * c.bn * 512 > ring)) break;
       const long long at_once = s > 1 ? tiles : sm_count / c.cg;
       const int blocks = s > 1 ? (k_stages + s - 1) / s * per : K / 128;
       const double mma = blocks * (M <= 128 ? c.few_us : c.many_us);
@@ -77,6 +82,49 @@ Tiling choose_tiling(int M, int N, int K, bool gated, int sm_count, int smem_opt
     }
   }
   return best;
+}
+
+// A cluster lives in one GPC, and how many SMs of a GPC are in use differs from device to device.  No more than seven eighths of
+// the SMs are counted on in any case.
+void cluster_limits(int sm_count, int (&clusters)[3]) {
+  for (int i = 0; i < 3; ++i) clusters[i] = (sm_count - sm_count / 8) >> (i + 1);
+}
+int clusters_at_once(const fg::host::Device& dev, int (&clusters)[3]) {
+  static std::mutex mu;
+  static std::map<int, std::array<int, 3>>* known = new std::map<int, std::array<int, 3>>;
+  std::lock_guard<std::mutex> lk(mu);
+  const auto it = known->find(dev.index);
+  cluster_limits(dev.sm_count, clusters);
+  if (it == known->end()) {
+    // (Every tiling's ring takes an SM's shared memory, so one kernel speaks for all.)
+    const auto kern = fg::fg_gemm8_kernel<1, 64>;
+    const int smem = fg::gemm8_smem_bytes(1, 64, stages_of({64, 1, 0.0, 0.0}, dev.smem_optin));
+    const int st = fg::host::opt_in_smem(reinterpret_cast<const void*>(kern), smem);
+    if (st != FG_OK) return st;
+    std::array<int, 3> found;
+    for (int i = 0; i < 3; ++i) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(dev.sm_count / (2 << i) * (2 << i));
+      cfg.blockDim = dim3(fg::kGemm8Threads);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 2 << i;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      const cudaError_t e = cudaOccupancyMaxActiveClusters(&found[i], kern, &cfg);
+      if (e != cudaSuccess) {
+        fg::host::launched(e);
+        return FG_ERR_CUDA;
+      }
+    }
+    known->emplace(dev.index, found);
+    for (int i = 0; i < 3; ++i) clusters[i] = clusters[i] < found[i] ? clusters[i] : found[i];
+  } else {
+    for (int i = 0; i < 3; ++i) clusters[i] = clusters[i] < it->second[i] ? clusters[i] : it->second[i];
+  }
+  return FG_OK;
 }
 
 template <int CG, int BN>
@@ -131,7 +179,7 @@ extern "C" int fg_linear_w8a8(const int8_t* x8, const int8_t* W8, const void* x_
       !aligned(w_scales, 2) || !aligned(bias, 2) || !aligned(status_dev, 4))
     return FG_ERR_ALIGN;
   fg::host::Device dev;
-  const int st = fg::host::current_device(&dev);
+  int st = fg::host::current_device(&dev);
   if (st != FG_OK) return st;
   fg::W8A8Params a = {};
   a.C = static_cast<__half*>(C);
@@ -147,7 +195,9 @@ extern "C" int fg_linear_w8a8(const int8_t* x8, const int8_t* W8, const void* x_
   a.status = status_dev;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (M <= fg::kGemv8MaxM) return run_gemv(a, x8, W8, s);
-  const Tiling t = choose_tiling(M, N, K, act == FG_ACT_SILU_GATE, dev.sm_count, dev.smem_optin);
+  int clusters[3];
+  if ((st = clusters_at_once(dev, clusters)) != FG_OK) return st;
+  const Tiling t = choose_tiling(M, N, K, act == FG_ACT_SILU_GATE, dev.sm_count, dev.smem_optin, clusters);
   if (t.cg == 2) return run_gemm<2, 256>(a, x8, W8, 1, dev, s);
   switch (t.bn) {
     case 32: return run_gemm<1, 32>(a, x8, W8, t.splits, dev, s);
@@ -159,8 +209,10 @@ extern "C" int fg_linear_w8a8(const int8_t* x8, const int8_t* W8, const void* x_
   }
 }
 
-// Internal (for the tests): the tiling of a call as bn | cg << 16 | splits << 24.
+// Internal (for the tests): the tiling of a call as bn | cg << 16 | splits << 24, as far as the device holds its clusters.
 extern "C" int fg_linear_w8a8_tiling(int M, int N, int K, int gated, int sm_count, int smem_optin) {
-  const Tiling t = choose_tiling(M, N, K, gated != 0, sm_count, smem_optin);
+  int clusters[3];
+  cluster_limits(sm_count, clusters);
+  const Tiling t = choose_tiling(M, N, K, gated != 0, sm_count, smem_optin, clusters);
   return t.bn | t.cg << 16 | t.splits << 24;
 }
