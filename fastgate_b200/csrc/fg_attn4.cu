@@ -7,9 +7,10 @@
 // so the matrix products run on bare codes and every scale is applied to a score or a weight, in 32 bits.
 //
 // The bytes of the cache are the floor: D + 8 of them per row and head, against 16 D bit operations' worth of
-// unpacking.  Measured on B200 (64 / 8 heads of 128 channels): 64 sequences of up to 8000 rows 93.6 us, 4.2 TB/s, with the tensor pipe
-// 38 % and the integer pipe 43 % busy: the latency of dependent instructions at two warps a scheduler bounds it.  One sequence of
-// 5000 rows (32 / 8 heads) 10.4 us: lengths, table, rows, partial sums, ticket, join, each a trip to L2 or memory.
+// unpacking.  Measured on B200 (64 / 8 heads of 128 channels): 64 sequences of up to 8000 rows 93.6 us, 4.2 TB/s.  Of the 500
+// cycles that a scheduler spends on 16 rows the tensor pipe is busy 192 and the integer pipe 220, and the two hardly overlap: more
+// warps do not help (twelve an SM 97 us; ten, three of them on one scheduler, 110).  One sequence of 5000 rows (32 / 8 heads)
+// 10.4 us: lengths, table, rows, partial sums, ticket, join, each a trip to L2 or memory.
 // What this kernel does about the unpacking:
 //   - A code's four bits, masked in place, ARE an fp16 number: bits 0-3 of a half are the subnormal code * 2^-24, bits 4-7
 //     code * 2^-20.  The tensor core multiplies subnormals exactly, so unpacking is one AND per two codes (and one shift
