@@ -6,8 +6,8 @@
 // format has.  2^-24 is the smallest positive fp16: a constant row gets it instead of a division by zero.
 //
 // Both kernels move each byte once.  Measured on B200: read 40000 rows of 8 heads of 128 channels 38.6 us (5.4 TB/s, nine
-// tenths of it stores), append 6001 tokens of 48 heads of 64 channels 17.1 us (3.9 TB/s: each lane waits for its slot, then for
-// its rows; issue slots are half full), and 64 tokens 2.3, 500 rows read 1.9 us, which is a launch and those latencies.
+// tenths of it stores), append 6001 tokens of 48 heads of 64 channels 16.6 us (4.0 TB/s: each lane waits for its slot, then for
+// its rows; issue slots are half full), and 64 tokens 2.1, 500 rows read 1.8 us, which is a launch and those latencies.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -18,7 +18,7 @@
 namespace fg {
 namespace {
 
-constexpr int kKvThreads = 256;
+constexpr int kKvThreads = 128;  // (6001 tokens appended: 16.6 us, with 256 17.1, with 384 17.8)
 
 struct AppendParams {
   const __half *q, *k, *v;       // token strides ldq, ldk, ldv; heads dense
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
     const int h = head0 + i;
     raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
     // One head: the row is asked for without waiting for its slot, also a padding token's (64 tokens: 2.3 us, else 2.5).  Four
-    // heads: after the slot (6001 tokens of 48 heads: 17.1 us, else 19.2).
+    // heads: after the slot (6001 tokens of 48 heads, 256 threads: 17.1 us, else 19.2).
     if ((HPT == 1 ? there : go) && h < heads) {
       const __half* src = h < p.q_heads ? p.q + token * p.ldq + static_cast<long long>(h) * D
                           : h < turned  ? p.k + token * p.ldk + static_cast<long long>(h - p.q_heads) * D
@@ -304,10 +304,10 @@ extern "C" int fg_kv_append_int4(const void* k, long long ldk, const void* v, lo
   p.kv = {static_cast<uint8_t*>(pages), num_pages, kv_heads, page_size};
   p.status = status_dev;
   p.tokens = tokens;
-  // Few rows: one a lane group, for latency; enough rows for two CTAs' worth a SM with four: four (6001 tokens of 48 heads of
-  // 64 channels: 17.1 us, with one 21.6; 64 tokens: 2.3 us, with four 4.7).
+  // Few rows: one a lane group, for latency; enough rows for four CTAs' worth a SM with four: four (6001 tokens of 48 heads of
+  // 64 channels: 16.6 us, with one 21.6; 64 tokens: 2.3 us, with four 4.7).
   const long long heads = q_heads + 2LL * kv_heads, rows_per_cta = kKvThreads / (d / 16);
-  const bool many = tokens * heads >= 4 * 4 * rows_per_cta * dev.sm_count;
+  const bool many = tokens * heads >= 4 * 8 * rows_per_cta * dev.sm_count;
   const long long gx = (tokens + rows_per_cta - 1) / rows_per_cta, gy = (heads + (many ? 3 : 0)) / (many ? 4 : 1);
   if (gx > 0x7fffffffLL || gy > 65535) return FG_ERR_SHAPE;
   void (*kern)(const AppendParams) = d == 128 ? (many ? fg_kv_append_kernel<128, 4> : fg_kv_append_kernel<128, 1>)
@@ -335,7 +335,7 @@ extern "C" int fg_kv_read_int4(const void* pages, long long num_pages, int page_
   p.status = status_dev;
   p.tokens = tokens;
   const long long rows_per_cta = kKvThreads / (d / 8), gx = (tokens + rows_per_cta - 1) / rows_per_cta;
-  const bool many = tokens * kv_heads >= 4 * 8 * rows_per_cta * dev.sm_count;  // 40000 rows: 38 us, with one head a thread 47
+  const bool many = tokens * kv_heads >= 4 * 16 * rows_per_cta * dev.sm_count;  // 40000 rows: 38 us, with one head a thread 47
   const long long gy = (kv_heads + (many ? 3 : 0)) / (many ? 4 : 1);
   if (gx > 0x7fffffffLL || gy > 65535) return FG_ERR_SHAPE;
   void (*kern)(const ReadParams) = d == 128 ? (many ? fg_kv_read_kernel<128, 4> : fg_kv_read_kernel<128, 1>)
