@@ -8,7 +8,8 @@
 //   CG = 2: two CTAs of a cluster share one 256 x 256 tile (cta_group::2).  Each loads its own 128 token rows and half of
 //           the tile's weight rows; the tensor cores of both read both halves of the weights.  A CTA alone at 128 x 256
 //           would fetch 48 KB from L2 per 128 k for the same 128 x 256 products, the pair fetches 32 KB per CTA, which is
-//           what L2 can deliver at full tensor rate.  One thread of the leading CTA issues every MMA.
+//           what L2 can deliver at full tensor rate.  One thread of the leading CTA issues every MMA.  The last columns of
+//           tiles may be narrower, so that the last wave of pairs is no longer than it has to be.
 //   CG = 1: one CTA per 128 x BN tile.  BN (32 to 256) is chosen so that the tiles of a small problem fill the card: the
 //           token rows beyond M cost no traffic and, next to the weight, no time.  Where even the narrowest tiles are too few,
 //           a cluster of 2 to 8 CTAs shares one, each with its part of k: the followers push their sums into the leader's
@@ -17,7 +18,7 @@
 // Persistent: CTAs (pairs) take tiles blockIdx.x, + gridDim.x, ... with the token tiles innermost, so that the tiles in
 // flight share weight rows in L2.  Two accumulators alternate: the epilogue of one tile overlaps the MMAs of the next.
 // The first ring-full of weights is asked for before the previous kernel of the stream has finished (the weight depends
-// on no kernel).  Measured on B200: 3001 x 4096 x 11008 100 us (2.7 POP/s; 192 pair tiles on 74 pairs are 2.6 waves and take three),
+// on no kernel).  Measured on B200: 3001 x 4096 x 11008 99 us (2.7 POP/s: two waves of 74 pairs and one of narrower tiles),
 // 16 x 28672 x 8192 with the SiLU gate 41 us (5.8 TB/s).  Warps 0-3: epilogue (TMEM lane = token row), 4: copies, 5: MMA.
 // Sums are exact 32-bit integers.
 #pragma once
@@ -31,6 +32,7 @@ constexpr int kGemm8Threads = 192;
 struct Gemm8Params {
   W8A8Params out;
   int tiles_m, tiles_n;
+  int wide, narrow;          // CG = 2: the first `wide` columns of tiles have BN weight rows, the others `narrow` (a multiple of 64)
   int stages;
   int splits;                // CG = 1: CTAs of a cluster that share a tile, each with its part of k (1: none)
   int x_rows;                // token rows of one copy: 128, or fewer when M is below (the tile's other rows are left as they are:
@@ -134,7 +136,8 @@ __device__ __forceinline__ void load_sums(uint32_t taddr, uint32_t (&r)[PIECE]) 
 
 template <int CG, int BN>
 __global__ void __launch_bounds__(kGemm8Threads, 1)
-    fg_gemm8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const Gemm8Params p) {
+    fg_gemm8_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                    const __grid_constant__ CUtensorMap tmNarrow, const Gemm8Params p) {
   constexpr int kBlock = gemm8_block_bytes(CG, BN), kPer = gemm8_blocks_per_stage(CG, BN), kStage = kPer * kBlock;
   constexpr uint32_t kCols = gemm8_tmem_cols(BN);
   constexpr int kPiece = BN >= 64 ? 32 : 16;       // columns that the epilogue takes at a time
@@ -191,6 +194,11 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
   const int tiles = p.tiles_m * p.tiles_n, groups = gridDim.x / cluster, group = blockIdx.x / cluster;
   const int k_blocks = p.out.K / 128, all_stages = (k_blocks + kPer - 1) / kPer;
   const int ks0 = part * all_stages / splits, ks1 = (part + 1) * all_stages / splits;  // this CTA's stages of every tile
+  auto first_of = [&](int tn) {  // first weight row of a column of tiles
+    if (CG == 2 && tn > p.wide) return p.wide * BN + (tn - p.wide) * p.narrow;
+    return tn * BN;
+  };
+  auto width_of = [&](int tn) { return CG == 2 && tn >= p.wide ? p.narrow : BN; };
   bool dead = false;
   auto report = [&] {
     if (p.out.status != nullptr) atomicExch(p.out.status, kStatusTimeout);
@@ -198,7 +206,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
 
   // Epilogue of a warp's 32 token rows of a tile (TMEM buffer b): scales, bias, activation, residual, kPiece columns at a time; a
   // row's pieces leave as 16-byte stores.  more: followers' sums, [splits - 1][BN][128], or nullptr.
-  auto finish = [&](int n0, int m, bool row, float xs, uint32_t b, const uint32_t* more) {
+  auto finish = [&](int n0, int bn, int m, bool row, float xs, uint32_t b, const uint32_t* more) {
     const W8A8Params& q = p.out;
     const int width = gated ? q.N >> 1 : q.N;
     if (!__any_sync(0xffffffffu, row)) return;  // a small M: nothing to store for these rows
@@ -239,7 +247,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
       // kHalf gate columns, then the matching up columns, per block of 2 kHalf
       constexpr int kHalf = BN < 128 ? BN / 2 : 64;
 #pragma unroll 1
-      for (int c = 0; c < BN / 2; c += kPiece) {  // column of the tile's output
+      for (int c = 0; c < bn / 2; c += kPiece) {  // column of the tile's output
         const int at = c / kHalf * (2 * kHalf) + c % kHalf;
         uint32_t g[kPiece], u[kPiece];
         load_piece(at, g);
@@ -254,7 +262,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
       with_act(q.act, [&](auto tag) {
         constexpr int ACT = decltype(tag)::value;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += kPiece) {
+        for (int c = 0; c < bn; c += kPiece) {
           uint32_t r[kPiece];
           load_piece(c, r);
           if (n0 + c >= q.N) continue;
@@ -274,12 +282,13 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
     const uint64_t pol_w = p.tiles_m > 1 ? policy_evict_last() : policy_evict_first();
     const bool two_boxes = BN < 128 && gated;
     const uint32_t full0 = CG == 2 ? map_to_rank(bar_full, 0) : bar_full;  // barriers of the leading CTA
-    int m_row = 0, n_row = 0;  // first token row and weight row of this CTA's copies
+    int m_row = 0, n_row = 0, bn = BN;  // first token row and weight row of this CTA's copies, the tile's width
     auto enter = [&](int t) {
-      const int tn = t / p.tiles_m, n0 = tn * BN;
+      const int tn = t / p.tiles_m, n0 = first_of(tn);
+      bn = width_of(tn);
       m_row = (t - tn * p.tiles_m) * (128 * CG) + 128 * static_cast<int>(rank);
       // with the gate and less than a block of 128: output columns n0 / 2 .., gate rows here, up rows 64 further on
-      n_row = two_boxes ? (n0 / 2 / 64) * 128 + n0 / 2 % 64 : n0 + (BN / CG) * static_cast<int>(rank);
+      n_row = two_boxes ? (n0 / 2 / 64) * 128 + n0 / 2 % 64 : n0 + (bn / CG) * static_cast<int>(rank);
     };
     auto load_x = [&](int slot, int ks) {
 #pragma unroll
@@ -294,7 +303,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
     };
     auto load_w = [&](int slot, int ks) {
       const int blocks = k_blocks - ks * kPer < kPer ? k_blocks - ks * kPer : kPer;
-      if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * slot, CG * blocks * (kBlock - (128 - p.x_rows) * 128));
+      if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * slot, CG * blocks * (kBlock - (128 - p.x_rows + (BN - bn) / CG) * 128));
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int kb = ks * kPer + i;
@@ -304,7 +313,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
             tma_load_2d(dst, &tmW, full0 + 8 * slot, kb * 128, n_row, pol_w);
             if (two_boxes) tma_load_2d(dst + BN / 2 * 128, &tmW, full0 + 8 * slot, kb * 128, n_row + 64, pol_w);
           } else {
-            tma_load_2d_pair(dst, &tmW, full0 + 8 * slot, kb * 128, n_row, pol_w);
+            tma_load_2d_pair(dst, bn == BN ? &tmW : &tmNarrow, full0 + 8 * slot, kb * 128, n_row, pol_w);
           }
         }
       }
@@ -352,7 +361,6 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
     // ------------------------------------ MMA ------------------------------------
     if (rank == 0) {
       const bool one = elect_one();
-      constexpr uint32_t idesc = umma_idesc_i8(128 * CG, BN);
       constexpr uint64_t desc = umma_smem_desc(0, 1, 64);
       int s = 0, n = 0;
       uint32_t ph = 0;
@@ -363,7 +371,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
           break;
         }
         tc_fence_after_sync();
-        const uint32_t acc = tmem_base + b * BN;
+        const uint32_t acc = tmem_base + b * BN, idesc = umma_idesc_i8(128 * CG, width_of(t / p.tiles_m));
         for (int ks = ks0; ks < ks1; ++ks) {
           if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar_full + 8 * s, ph, kWaitBudgetNs))) {
             dead = true;
@@ -399,12 +407,13 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
     const W8A8Params& q = p.out;
     int n = 0;
     for (int t = group; t < tiles; t += groups, ++n) {
-      const int m = (t % p.tiles_m) * (128 * CG) + 128 * rank + 32 * warp + lane, n0 = (t / p.tiles_m) * BN;
+      const int m = (t % p.tiles_m) * (128 * CG) + 128 * rank + 32 * warp + lane, n0 = first_of(t / p.tiles_m);
+      const int bn = width_of(t / p.tiles_m);
       const uint32_t b = n & 1, use = n >> 1;
       const bool row = m < q.M;
       const float xs = row ? x_scale(q, m) : 0.f;
       named_bar_sync(1, 128);  // the previous tile's column values have been read
-      for (int j = threadIdx.x; j < BN; j += 128) {
+      for (int j = threadIdx.x; j < bn; j += 128) {
         int w = n0 + j;  // weight row of column j
         if (BN < 128 && gated) w = gate_row(n0 / 2 + j % (BN / 2)) + (j < BN / 2 ? 0 : 64);
         col_scale[j] = w < q.N && q.w_scales != nullptr ? __half2float(q.w_scales[w]) : 1.f;
@@ -418,7 +427,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
       if (CG == 1 && splits > 1) break;  // the cluster's one tile: finished below, together
       if (dead) continue;
       tc_fence_after_sync();
-      finish(n0, m, row, xs, b, nullptr);
+      finish(n0, bn, m, row, xs, b, nullptr);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
@@ -453,7 +462,7 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
         const int m = (group % p.tiles_m) * 128 + 32 * warp + lane;
         const bool row = m < p.out.M;
         tc_fence_after_sync();
-        finish(group / p.tiles_m * BN, m, row && !dead, row ? x_scale(p.out, m) : 0.f, 0, reinterpret_cast<const uint32_t*>(smem_gen) + 32 * warp + lane);
+        finish(group / p.tiles_m * BN, BN, m, row && !dead, row ? x_scale(p.out, m) : 0.f, 0, reinterpret_cast<const uint32_t*>(smem_gen) + 32 * warp + lane);
       }
     }
   }

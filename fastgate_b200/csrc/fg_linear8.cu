@@ -35,6 +35,8 @@ struct Tiling {
   int bn;      // weight rows of a tile
   int cg;      // CTAs that share a tile's MMAs: 1 (128 token rows) or 2 (256)
   int splits;  // CTAs that share a tile's k (cg 1)
+  int wide;    // cg 2: columns of tiles of full width; the others have `narrow` weight rows
+  int narrow;
 };
 
 struct TileCost {
@@ -45,6 +47,7 @@ struct TileCost {
 // blocks of k.  Narrow tiles are bound by the issue of their four MMAs a block, wide ones by the tensor cores and L2.
 constexpr TileCost kTileCosts[] = {{32, 1, 0.148, 0.155}, {64, 1, 0.163, 0.18}, {96, 1, 0.175, 0.21}, {128, 1, 0.22, 0.25},
                                    {192, 1, 0.265, 0.32}, {256, 1, 0.36, 0.40}, {256, 2, 0.36, 0.36}};
+constexpr double kNarrowUs[] = {0.17, 0.22, 0.28};  // the same of a pair's tile with 64, 128 and 192 weight rows
 constexpr double kSplitUs = 3.5;    // launch of clusters, two cluster barriers and the exchange between them
 constexpr double kDramBytesPerUs = 6.2e6;
 
@@ -58,7 +61,7 @@ int stages_of(const TileCost& c, int smem_optin) {
 // clusters: how many clusters of 2, 4 and 8 CTAs the device holds at once.
 Tiling choose_tiling(int M, int N, int K, bool gated, int sm_count, int smem_optin, const int (&clusters)[3]) {
   const double dram = (static_cast<double>(N) * K + static_cast<double>(M) * K + 2.0 * M * N) / kDramBytesPerUs;
-  Tiling best = {128, 1, 1};
+  Tiling best = {128, 1, 1, 0, 0};
   double best_us = 1e30;
   for (const TileCost& c : kTileCosts) {
     if (gated && (c.bn == 96 || c.bn == 192)) continue;  // a gate row and its up row belong to one tile
@@ -77,7 +80,26 @@ Tiling choose_tiling(int M, int N, int K, bool gated, int sm_count, int smem_opt
       const double us = full * (mma > full_dram ? mma : full_dram) + (rest ? (mma > rest_dram ? mma : rest_dram) : 0.0) + (s > 1 ? kSplitUs : 0.0);
       if (us < best_us) {
         best_us = us;
-        best = {c.bn, c.cg, s};
+        best = {c.bn, c.cg, s, (N + c.bn - 1) / c.bn, c.bn};
+      }
+    }
+  }
+  // Pairs: a last wave that is far from full may be a wave of narrower tiles instead.  (A row of tiles spans the waves: what counts is
+  // how many waves have a wide tile in them and how many have none.  512 x 28672 x 8192: 98.6 us with wide tiles alone, 90.7;
+  // 512 x 11008 x 4096: 25.0 / 23.2; 3001 x 4096 x 11008: 100 / 98.8.)
+  const int pairs = sm_count / 2, tiles_m = (M + 255) / 256, blocks = K / 128;
+  for (int i = 0; i < 3; ++i) {
+    const int narrow = 64 * (i + 1);
+    if (gated && narrow != 128) continue;
+    for (int wide = N / 256; wide >= 0 && wide >= N / 256 - 64; --wide) {
+      const long long wide_tiles = static_cast<long long>(tiles_m) * wide, tiles = wide_tiles + static_cast<long long>(tiles_m) * ((N - 256 * wide + narrow - 1) / narrow);
+      if (tiles == wide_tiles || wide_tiles < pairs) continue;
+      const long long wide_waves = (wide_tiles + pairs - 1) / pairs, waves = (tiles + pairs - 1) / pairs;
+      double us = blocks * (wide_waves * 0.36 + (waves - wide_waves) * kNarrowUs[i]);
+      if (us < dram) us = dram;
+      if (us < 0.98 * best_us) {
+        best_us = us;
+        best = {256, 2, 1, wide, narrow};
       }
     }
   }
@@ -128,7 +150,8 @@ int clusters_at_once(const fg::host::Device& dev, int (&clusters)[3]) {
 }
 
 template <int CG, int BN>
-int run_gemm(const fg::W8A8Params& a, const int8_t* x, const int8_t* W, int splits, const fg::host::Device& dev, cudaStream_t stream) {
+int run_gemm(const fg::W8A8Params& a, const int8_t* x, const int8_t* W, const Tiling& t, const fg::host::Device& dev, cudaStream_t stream) {
+  const int splits = t.splits;
   const auto kern = fg::fg_gemm8_kernel<CG, BN>;
   const int stages = stages_of({BN, CG, 0.0, 0.0}, dev.smem_optin);
   if (stages < 2) return FG_ERR_PLAN;
@@ -137,13 +160,19 @@ int run_gemm(const fg::W8A8Params& a, const int8_t* x, const int8_t* W, int spli
   if (st != FG_OK) return st;
   const int x_rows = CG == 1 && a.M < 128 ? (a.M + 7) / 8 * 8 : 128;
   const int w_rows = fg::gemm8_box_rows(CG, BN, a.act == FG_ACT_SILU_GATE);
-  CUtensorMap tmW, tmX;
+  const int wide = CG == 2 ? t.wide : (a.N + BN - 1) / BN, narrow = CG == 2 ? t.narrow : BN;
+  CUtensorMap tmW, tmX, tmNarrow;
   if ((st = fg::host::encode_tensor(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, a.K, a.M, 128, x_rows)) != FG_OK) return st;
   if ((st = fg::host::encode_tensor(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, W, a.K, a.N, 128, w_rows)) != FG_OK) return st;
+  tmNarrow = tmW;
+  if (narrow != BN && (st = fg::host::encode_tensor(&tmNarrow, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, W, a.K, a.N, 128, narrow / CG)) != FG_OK) return st;
   fg::Gemm8Params p = {};
   p.out = a;
   p.tiles_m = (a.M + 128 * CG - 1) / (128 * CG);
-  p.tiles_n = (a.N + BN - 1) / BN;
+  const int rest = a.N - wide * BN;  // (of full columns alone the last may reach over N)
+  p.tiles_n = wide + (rest > 0 ? (rest + narrow - 1) / narrow : 0);
+  p.wide = wide;
+  p.narrow = narrow;
   p.stages = stages;
   p.splits = splits;
   p.x_rows = x_rows;
@@ -164,7 +193,7 @@ int run_gemm(const fg::W8A8Params& a, const int8_t* x, const int8_t* W, int spli
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster == 1 ? 1 : 2;
-  return fg::host::launched(cudaLaunchKernelEx(&cfg, kern, tmX, tmW, p));
+  return fg::host::launched(cudaLaunchKernelEx(&cfg, kern, tmX, tmW, tmNarrow, p));
 }
 
 }  // namespace
@@ -198,14 +227,14 @@ extern "C" int fg_linear_w8a8(const int8_t* x8, const int8_t* W8, const void* x_
   int clusters[3];
   if ((st = clusters_at_once(dev, clusters)) != FG_OK) return st;
   const Tiling t = choose_tiling(M, N, K, act == FG_ACT_SILU_GATE, dev.sm_count, dev.smem_optin, clusters);
-  if (t.cg == 2) return run_gemm<2, 256>(a, x8, W8, 1, dev, s);
+  if (t.cg == 2) return run_gemm<2, 256>(a, x8, W8, t, dev, s);
   switch (t.bn) {
-    case 32: return run_gemm<1, 32>(a, x8, W8, t.splits, dev, s);
-    case 64: return run_gemm<1, 64>(a, x8, W8, t.splits, dev, s);
-    case 96: return run_gemm<1, 96>(a, x8, W8, t.splits, dev, s);
-    case 128: return run_gemm<1, 128>(a, x8, W8, t.splits, dev, s);
-    case 192: return run_gemm<1, 192>(a, x8, W8, t.splits, dev, s);
-    default: return run_gemm<1, 256>(a, x8, W8, t.splits, dev, s);
+    case 32: return run_gemm<1, 32>(a, x8, W8, t, dev, s);
+    case 64: return run_gemm<1, 64>(a, x8, W8, t, dev, s);
+    case 96: return run_gemm<1, 96>(a, x8, W8, t, dev, s);
+    case 128: return run_gemm<1, 128>(a, x8, W8, t, dev, s);
+    case 192: return run_gemm<1, 192>(a, x8, W8, t, dev, s);
+    default: return run_gemm<1, 256>(a, x8, W8, t, dev, s);
   }
 }
 

@@ -211,6 +211,25 @@ def test_refusals(dev):
     assert args(act=9) == capi.FG_ERR_PLAN and args(xs=None) == capi.FG_ERR_NULL
 
 
+@pytest.mark.parametrize("M,N,K,act", [(3001, 4096, 1024, "none"), (2048, 5120, 1152, "gelu_tanh"), (3001, 3456, 1024, "none"), (4096, 4096, 1024, "silu_gate"),
+                                       (1500, 8192, 1024, "silu")])
+def test_last_columns_of_tiles_may_be_narrower(M, N, K, act, dev):
+    """Sizes whose last wave of wide tiles would be far from full: narrower ones of 64, 128 or 192 weight rows take its place."""
+    x8, w8, xs, ws, g = _data(M, N, K, M + N)
+    bias = torch.randn(N, generator=g).half()
+    width = N // 2 if act == "silu_gate" else N
+    res = torch.randn(M, width, generator=g).half()
+    d = [t.to(dev) for t in (x8, w8, xs, ws, bias, res)]
+    c = torch.full((M, width), float("nan"), dtype=torch.half, device=dev)
+    fg.linear_int8(d[0], d[1], c, d[2], d[3], d[4], d[5], act)
+    rows = torch.cat([torch.arange(0, M, 97), torch.arange(M - 3, M)])
+    _check(c[rows.to(dev)], *ref.linear_int8(x8[rows], w8, xs[rows], ws, bias, res[rows], act))
+    again = torch.empty_like(c)  # every row, bit for bit, against calls of other tilings
+    for m in range(0, M, 100):
+        fg.linear_int8(d[0][m:m + 100], d[1], again[m:m + 100], d[2][m:m + 100], d[3], d[4], d[5][m:m + 100], act)
+    assert torch.equal(c, again)
+
+
 def test_captured_before_any_eager_call(dev):
     """A stream's first call may be a captured one; the status word that it holds is the one that workspace_status() reads."""
     x8, w8, xs, ws, *_ = _data(9, 256, 512, 77)
