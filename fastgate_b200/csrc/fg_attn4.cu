@@ -223,8 +223,8 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) fg_kv_attention_
   if (lane < S) mbar_init(bar + 8 * lane, 1);
   fence_mbar_init();
   fence_proxy_async();
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
 
   // ---- this CTA's share [ub, ue) of the work list: equal runs of `chunk` units ----
   const int kv_heads = p.kv.heads;

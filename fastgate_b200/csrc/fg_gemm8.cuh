@@ -187,9 +187,11 @@ __global__ void __launch_bounds__(kGemm8Threads, 1)
   if (cluster > 1) cluster_sync();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot_gen;
-  griddep_launch_dependents();
   const bool gated = p.out.act == kActSiluGate;
-  if (warp != 4) griddep_wait();
+  if (warp != 4) {
+    griddep_wait();
+    griddep_launch_dependents();
+  }
 
   const int tiles = p.tiles_m * p.tiles_n, groups = gridDim.x / cluster, group = blockIdx.x / cluster;
   const int k_blocks = p.out.K / 128, all_stages = (k_blocks + kPer - 1) / kPer;

@@ -233,7 +233,6 @@ __global__ void __launch_bounds__((kGemvMaxWarps + 1) * 32, 1) fg_gemv_kernel(co
         mbar_arrive_expect_tx(bar_base + 8 * s, bytes);
         bulk_load_1d(ring_base + s * p.stage_bytes, Wb + static_cast<size_t>(row0) * row_bytes, bytes, bar_base + 8 * s, pol_w);
       };
-      griddep_launch_dependents();
       int row = blockIdx.x * p.static_rows;
       const int end = row + p.static_rows;
       int s = 0;
@@ -253,6 +252,7 @@ __global__ void __launch_bounds__((kGemvMaxWarps + 1) * 32, 1) fg_gemv_kernel(co
         for (uint32_t o = 0; o < n; o += 16384) bulk_prefetch_l2(src + o, (n - o) < 16384u ? (n - o) : 16384u);
       }
       griddep_wait();
+      griddep_launch_dependents();
       if (trace) trace[14] = globaltimer_ns();
       // x may be read now.  The consumer warps fetch it with ordinary loads: a bulk copy would
       // queue in this SM's copy engine behind the ring-full of weight rows requested above.

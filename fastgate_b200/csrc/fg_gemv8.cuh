@@ -39,7 +39,6 @@ __global__ void __launch_bounds__(kGemv8Warps * 32) fg_gemv8_kernel(const Gemv8P
   for (int r = 0; r < R; ++r) {
     n[r] = gated && R > 1 ? gate_row(first / 2 + r / 2) + (r & 1) * 64 : first + r;
   }
-  griddep_launch_dependents();
   if (first >= N) return;
   const int pieces = K / 16;
   const uint4* w[R];
@@ -61,6 +60,7 @@ __global__ void __launch_bounds__(kGemv8Warps * 32) fg_gemv8_kernel(const Gemv8P
   };
   load(lane);
   griddep_wait();
+  griddep_launch_dependents();
   for (int at = lane; at < pieces;) {
 #pragma unroll
     for (int i = 0; i < kGemv8Pieces; ++i) {

@@ -571,7 +571,6 @@ __device__ __forceinline__ void run_producer(const CUtensorMap& tmW, const CUten
   // was still draining) or of a layer that other ranks are still pushing, so they are
   // only read after griddepcontrol.wait (a no-op for an ordinary launch) and, if asked,
   // after the arrival counters of that layer have reached their target.
-  griddep_launch_dependents();
   const int pre = n_it < S ? n_it : S;
   {
     int t2 = tile, k2 = kb;
@@ -604,6 +603,7 @@ __device__ __forceinline__ void run_producer(const CUtensorMap& tmW, const CUten
     }
   }
   griddep_wait();
+  griddep_launch_dependents();
   // after the wait: every earlier launch of the stream, including one that still compared these
   // buffers' counters with the old total, has completed
   if (blockIdx.x == 0 && p.target_dev != nullptr) atomicAdd(p.target_dev, static_cast<unsigned long long>(p.tiles));
@@ -1001,14 +1001,14 @@ __global__ void __launch_bounds__(streamk_max_threads<OP, MT>(), 1)
 // Waits (bounded) until each of the `world` per-source arrival counters of this rank has
 // reached `target`, i.e. until every rank has delivered all its tiles of the calls enqueued so
 // far.  One thread; ordered on the stream, so whatever follows it sees the complete output.
-// Launched with programmatic stream serialization: the launch after it may start at once (a GEMM
+// Launched with programmatic stream serialization: this kernel starts early and begins to look at the
+// counters once everything before it in the stream is done; from then on the launch after it may start too (a GEMM
 // then streams its first weight tiles while this kernel still waits; it touches nothing else before
-// its own griddepcontrol.wait, which returns when this kernel has completed), and this kernel itself
-// starts early and begins to look at the counters once everything before it in the stream is done.
+// its own griddepcontrol.wait, which returns when this kernel has completed).
 static __global__ void fg_push_wait_kernel(const unsigned long long* flags, int world, unsigned long long target,
                                     int* status) {
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
   if (threadIdx.x != 0) return;
   if (!wait_counters(flags, world, target)) atomicExch(status, kStatusTimeout);
 }
@@ -1016,8 +1016,8 @@ static __global__ void fg_push_wait_kernel(const unsigned long long* flags, int 
 // in *target_dev): nothing in the launch changes from call to call, so it can be replayed in a graph.
 static __global__ void fg_push_wait_dev_kernel(const unsigned long long* flags, int world,
                                         const unsigned long long* target_dev, int* status) {
-  griddep_launch_dependents();
   griddep_wait();  // the launches that add to *target_dev have completed
+  griddep_launch_dependents();
   if (threadIdx.x != 0) return;
   const unsigned long long target = __ldcg(target_dev);
   if (!wait_counters(flags, world, target)) atomicExch(status, kStatusTimeout);
@@ -1032,8 +1032,8 @@ struct WaitList {
   int count;
 };
 static __global__ void fg_push_wait_many_kernel(const WaitList w, int world, int* status) {
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
   const int i = threadIdx.x;
   if (i >= w.count) return;
   if (!wait_counters(w.flags[i], world, __ldcg(w.target_dev[i]))) atomicExch(status, kStatusTimeout);

@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(kKvThreads) fg_kv_append_kernel(const AppendPa
   const int heads = p.q_heads + 2 * p.kv.heads, turned = p.q_heads + p.kv.heads;  // head numbers below `turned` are rotated
   const long long token = static_cast<long long>(blockIdx.x) * (kKvThreads / LPR) + threadIdx.x / LPR;
   const int head0 = blockIdx.y * HPT;
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
 
   // A padding token (negative slot) is left out whole; an index out of range too, and reported.
   const bool there = token < p.tokens;

@@ -86,8 +86,8 @@ __global__ void __launch_bounds__(kNormMaxThreads) fg_add_rmsnorm_kernel(const N
   const __half* x = p.x + row * p.ldx;
   const ResT* res = static_cast<const ResT*>(p.residual) + row * p.K;
   ResT* res_out = static_cast<ResT*>(p.residual_out) + row * p.K;
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
 
   auto load_h = [&](int v, float (&h)[8]) {
     load8(x + 8 * v, h);

@@ -163,6 +163,9 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 }
 
 // Programmatic dependent launch (no-ops when the kernel was launched without the attribute).
+// Every kernel signals its dependents after its own wait, never before: the next launch then starts only once everything in
+// front of this kernel has completed, and what it reads before its own wait (weights) can be unfinished only if the kernel
+// directly in front of it writes it.  Signalled before the wait, launches would start any number of kernels ahead.
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddep_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -246,7 +246,6 @@ __global__ void __launch_bounds__(kUmmaGroupThreads, 1) fg_umma_group_kernel(con
       };
       if (trace) trace[1] = globaltimer_ns();
       // weights first (they never depend on earlier kernels), activations after the wait
-      griddep_launch_dependents();
       const int pre = n_it < S ? n_it : S;
       for (int i = 0; i < pre; ++i) {
         acquire(cw);
@@ -256,6 +255,7 @@ __global__ void __launch_bounds__(kUmmaGroupThreads, 1) fg_umma_group_kernel(con
         cursor_advance(g, cw, 1);
       }
       griddep_wait();
+      griddep_launch_dependents();
       if (blockIdx.x == 0 && g.target_dev != nullptr) atomicAdd(g.target_dev, static_cast<unsigned long long>(g.total_tiles));
       for (int i = 0; i < pre; ++i) {
         issue_x(i, cx, stage_chunks(cx));

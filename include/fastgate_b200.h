@@ -392,7 +392,8 @@ int fg_add_rmsnorm(const void* x, long long ldx, const void* weight, const void*
  * x_scales fp32 (x_scales_f32 == 1) or fp16; bias [N], residual and C fp16; act FG_ACT_*.  With FG_ACT_SILU_GATE W8 holds 64
  * gate rows, then the matching 64 up rows, per 128 (fg_prepack_gate_up_w8; w_scales and bias in the same order); C and
  * residual are [M, N/2].  The sums are exact 32-bit integers: a row's result depends neither on the rows beside it nor on how
- * the work is split.  W8 may be read before the kernel in front of the call has finished: it must not be what that kernel writes.
+ * the work is split.  W8 may be read before the call directly in front on the stream has finished: it must not be what that call writes
+ * (what calls before that one write is complete).
  * K, N % 128 == 0, K <= 130944 (where the sums still fit), any M >= 1.  residual may be C.  No workspace;
  * *status_dev (int in device memory, or NULL: not reported) gets FG_ERR_TIMEOUT if a bounded wait gave up. */
 int fg_linear_w8a8(const int8_t* x8, const int8_t* W8, const void* x_scales, int x_scales_f32, const void* w_scales, void* C,
