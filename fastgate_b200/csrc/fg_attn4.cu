@@ -720,8 +720,9 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) fg_kv_attention_
 
   // ---- items of several CTAs: the last of them to get here joins the partials in CTA order ----
   if (n_pending > 0) {
+    // The thread that took the tickets acquires what the other CTAs released with theirs, the barrier carries it to all threads.
+    if (tid == 0) fence_acq_rel_gpu();
     __syncthreads();
-    fence_acq_rel_gpu();
   }
   for (int k = 0; k < n_pending; ++k) {
     const Pending q = pending[k];

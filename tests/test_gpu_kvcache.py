@@ -456,3 +456,28 @@ def test_refusals(dev):
                                                None, kw.get("ws", ws.data_ptr()), ws.numel(), vp(0))
     assert call(ldq=100) == call(d=96) == call(page=8) == call(batch=3) == call(scale=-1.0) == capi.FG_ERR_SHAPE
     assert call(ws=None) == call(ws=ws.data_ptr() + 16) == capi.FG_ERR_WORKSPACE
+
+
+def test_joins_read_the_partials_of_their_own_call(dev):
+    """Items of several CTAs, call after call on one stream and over other rows each time: whoever joins an item adds up the partial sums
+    that its partners have just left in the workspace, not those of the call before."""
+    page, d = 64, 128
+    lens = [5000, 1800, 300]
+    cases = []
+    for seed in range(4):
+        pool, table, q, _ = _case(lens, None, 8, 2, d, page, 100 + seed)
+        cases.append((pool, table, q, [t.to(dev) for t in (pool, table, q)]))
+    ld = torch.tensor(lens, dtype=torch.int32, device=dev)
+    want = []
+    for pool, table, q, (pd, td, qd) in cases:
+        out = torch.empty_like(qd)
+        fg.kv_attention_int4(qd, pd, td, ld, out, page)
+        torch.cuda.synchronize()
+        _check_attention(out, pool, table, q, lens, page, None)
+        want.append(out)
+    got = [torch.empty_like(want[0]) for _ in range(400)]
+    for i, out in enumerate(got):
+        _, _, _, (pd, td, qd) = cases[i % 4]
+        fg.kv_attention_int4(qd, pd, td, ld, out, page)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[i % 4]) for i, out in enumerate(got))
