@@ -76,6 +76,13 @@ __device__ __forceinline__ void store8(int8_t* p, const float (&v)[8]) {
   *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 
+// The larger of two values, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // RES: 0 none, 1 fp16, 2 fp32.  VPT: vectors of eight elements a thread keeps; 0: a row too long for the
 // registers, read a second time (from L2) instead.
 template <int RES, bool INT8, int VPT>
@@ -106,7 +113,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) fg_add_rmsnorm_kernel(const N
     for (int i = 0; i < 8; ++i) {
       sum = fmaf(h[i], h[i], sum);
       h[i] = __fmul_rn(h[i], w[i]);
-      if (INT8) top = fmaxf(top, fabsf(h[i]));
+      if (INT8) top = max_nan(top, fabsf(h[i]));
     }
   };
   if constexpr (VPT > 0) {
@@ -136,7 +143,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) fg_add_rmsnorm_kernel(const N
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (INT8) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (INT8) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
   }
   if (threads > 32) {
     if ((tid & 31) == 0) part[tid >> 5] = make_float2(sum, top);
@@ -147,16 +154,16 @@ __global__ void __launch_bounds__(kNormMaxThreads) fg_add_rmsnorm_kernel(const N
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) {
       sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      if (INT8) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      if (INT8) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
     }
   }
   const float rstd = 1.f / sqrtf(sum / static_cast<float>(p.K) + p.eps);
   // The largest finite factor stands in for 127 / a where that overflows (a below 4e-37).
   const float factor = INT8 ? (top > 0.f ? fminf(__fdiv_rn(127.f, top), 3.402823466e38f) : 0.f) : rstd;
   if (INT8 && tid == 0) {
-    // fmaxf drops NaNs from `top`, but not from the sum: sum - sum is 0 unless a term was infinite or NaN
-    const float bad = sum - sum;
-    p.scales[row] = (top > 0.f ? top * rstd / 127.f : 1.f) + (bad == 0.f ? 0.f : __int_as_float(0x7fc00000));
+    // `top` is infinite or NaN if some t is, be it from the row or from the weight
+    const bool finite = top <= 3.402823466e38f && sum <= 3.402823466e38f;
+    p.scales[row] = finite ? (top > 0.f ? top * rstd / 127.f : 1.f) : __int_as_float(0x7fc00000);
   }
 
   auto emit = [&](int v, float (&t)[8]) {

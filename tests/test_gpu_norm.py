@@ -109,6 +109,25 @@ def test_rows_of_the_extremes(dev):
     assert bool(torch.isnan(y[3]).all())
 
 
+@pytest.mark.parametrize("K", [64, 1024, 40000])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_weights_that_are_not_finite_show_in_the_scale(bad, K, dev):
+    """Not finite is h * weight, whichever of the two is to blame, a zero times an infinity included; fp16 rows show it in its place."""
+    x, w, r = _data(5, K, torch.float32, K, dev)
+    at = K // 2 + 3
+    x[2], r[2] = 0, 0
+    w[at] = bad
+    q, s = torch.empty(5, K, dtype=torch.int8, device=dev), torch.zeros(5, device=dev)
+    fg.add_rmsnorm(x.to(dev), w.to(dev), q, r.to(dev), scales=s)
+    assert bool(torch.isnan(s).all())
+    y = torch.empty(5, K, dtype=torch.half, device=dev)
+    fg.add_rmsnorm(x.to(dev), w.to(dev), y, r.to(dev))
+    want = ref.rmsnorm(x, w, r)[0]
+    other = torch.arange(K) != at
+    assert not bool(torch.isfinite(y[:, at]).any()) and bool(torch.isfinite(y.cpu()[:, other]).all())
+    assert bool(((y.cpu().double() - want).abs() <= want.abs() * (ref.HALF_STEP + REL) + ref.TINY)[:, other].all())
+
+
 def test_refusals(dev):
     x = torch.zeros(2, 64, dtype=torch.half, device=dev)
     w = torch.ones(64, dtype=torch.half, device=dev)
