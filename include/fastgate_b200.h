@@ -378,10 +378,11 @@ int fg_quantize_rows_w8(const void* W, int8_t* W8, void* scales, int N, int K, f
  *     out[m] = rint(t * (127 / a)), scales[m] = a * rstd / 127   with t = h * weight, a = max|t|
  *                                               (out_int8 == 1: the activations of fg_linear_w8a8)
  * rstd cancels out of the int8 codes, so they do not depend on the order of the sum of squares.  A row whose t is
- * all zero gets codes 0 and scale 1 (as in fg_quantize_rows_w8); one with an infinity or a NaN gets a NaN scale.
+ * all zero gets codes 0 and scale 1 (as in fg_quantize_rows_w8); one whose t has an infinity or a NaN (from the row, from the
+ * weight, or a product beyond fp32) gets codes 0 and a NaN scale.  With eps = 0 a row of zeros has no fp16 value and gives NaN.
  * weight [K] fp16; residual and residual_out [M,K] dense, fp16 or (residual_f32 == 1) fp32, both NULL or neither; they
- * may be the same buffer.  An fp16 out may be x itself.  K % 8 == 0, M >= 1.  Sums in fp32.  No counterpart in the
- * reference (it has no norm). */
+ * may be the same buffer.  An fp16 out may be x itself.  K % 8 == 0, M >= 1.  Sums in fp32, for residuals up to fp32's largest
+ * values.  No counterpart in the reference (it has no norm). */
 int fg_add_rmsnorm(const void* x, long long ldx, const void* weight, const void* residual, void* residual_out,
                    int residual_f32, void* out, int out_int8, float* scales, int M, int K, float eps, fg_stream_t stream);
 

@@ -128,6 +128,28 @@ def test_weights_that_are_not_finite_show_in_the_scale(bad, K, dev):
     assert bool(((y.cpu().double() - want).abs() <= want.abs() * (ref.HALF_STEP + REL) + ref.TINY)[:, other].all())
 
 
+@pytest.mark.parametrize("K", [64, 4096, 40000])
+@pytest.mark.parametrize("size", [1e17, 1e19, 1e25, 4e37])
+def test_residuals_whose_squares_do_not_fit(size, K, dev):
+    """A residual stream in 32 bits far beyond the root of the largest number: finite rows give what the formula says."""
+    x, w, r = _data(6, K, torch.float32, 3, dev)
+    r = r.clamp(-7, 7) * size / 3
+    r[3] /= size  # an ordinary row between them
+    y, h, t, rstd = ref.rmsnorm(x, w, r, 1e-6)
+    out, rd = torch.empty(6, K, dtype=torch.half, device=dev), r.to(dev)
+    fg.add_rmsnorm(x.to(dev), w.to(dev), out, rd)
+    assert bool(((out.cpu().double() - y).abs() <= y.abs() * (ref.HALF_STEP + REL) + ref.TINY).all())
+    q, s = torch.empty(6, K, dtype=torch.int8, device=dev), torch.empty(6, device=dev)
+    fg.add_rmsnorm(x.to(dev), w.to(dev), q, r.to(dev), 1e-6, s)
+    _check_int8(q.cpu(), s.cpu(), t, rstd)
+    r[1, 5] = float("inf")
+    r[2, 7] = float("nan")
+    fg.add_rmsnorm(x.to(dev), w.to(dev), q, r.to(dev), 1e-6, s)
+    assert torch.isnan(s).tolist() == [False, True, True, False, False, False]
+    fg.add_rmsnorm(x.to(dev), w.to(dev), out, r.to(dev))
+    assert bool(torch.isnan(out[1, 5])) and bool((out[1] == 0).sum() == K - 1) and bool(torch.isnan(out[2]).all())
+
+
 def test_refusals(dev):
     x = torch.zeros(2, 64, dtype=torch.half, device=dev)
     w = torch.ones(64, dtype=torch.half, device=dev)
