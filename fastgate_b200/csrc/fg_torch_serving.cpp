@@ -77,6 +77,20 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
   return static_cast<const char*>(a.data_ptr()) < end(b) && static_cast<const char*>(b.data_ptr()) < end(a);
 }
 
+// The same for tensors of rows that are dense in themselves ([tokens, heads, channels], or anything dense): column ranges of one
+// buffer lie between each other's rows without meeting them.
+bool rows_overlap(const at::Tensor& a, const at::Tensor& b) {
+  if (!overlap(a, b)) return false;
+  if (a.dim() != 3 || b.dim() != 3 || a.size(0) < 2 || b.size(0) < 2 || a.element_size() != b.element_size() || a.stride(0) != b.stride(0)) return true;
+  const int64_t size = a.element_size(), step = a.stride(0) * size;
+  const int64_t wa = a.size(1) * a.size(2) * size, wb = b.size(1) * b.size(2) * size;
+  if (step < wa || step < wb) return true;
+  // where b's rows begin within a's period
+  const int64_t d = static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr());
+  const int64_t at = (d % step + step) % step;
+  return at < wa || at + wb > step;
+}
+
 // ---- RMS norm ------------------------------------------------------------------------------
 void add_rmsnorm(at::Tensor x, at::Tensor weight, at::Tensor out, OptTensor residual, double eps, OptTensor scales, OptTensor residual_out) {
   check_cuda(x, "x", at::kHalf, -1);
@@ -226,7 +240,9 @@ void kv_append_int4(at::Tensor k, at::Tensor v, at::Tensor pages, at::Tensor slo
     at::Tensor o = given(q_out) ? *q_out : *q;
     check_rows(o, "q_out", device);
     if (q->size(0) != T || q->size(2) != d || q->size(1) < 1 || o.sizes() != q->sizes()) bad_argument("q and q_out must be [tokens, q_heads, channels]");
-    if (overlap(o, *q) && !(o.data_ptr() == q->data_ptr() && row_stride(o) == row_stride(*q))) bad_argument("q_out may be q itself, but not overlap it otherwise");
+    if (rows_overlap(o, *q) && !(o.data_ptr() == q->data_ptr() && row_stride(o) == row_stride(*q))) bad_argument("q_out may be q itself, but not overlap it otherwise");
+    if (rows_overlap(o, k) || rows_overlap(o, v) || overlap(o, pages) || overlap(o, slots) || overlap(o, *cos_sin) || overlap(o, *positions))
+      bad_argument("q_out must not overlap k, v, pages, slots, cos_sin or positions");
     qp = q->data_ptr();
     qo = o.data_ptr();
     ldq = row_stride(*q);
@@ -235,6 +251,9 @@ void kv_append_int4(at::Tensor k, at::Tensor v, at::Tensor pages, at::Tensor slo
   } else if (given(q_out)) {
     bad_argument("q_out without q");
   }
+  if (overlap(pages, k) || overlap(pages, v) || overlap(pages, slots) || (given(q) && overlap(pages, *q)) ||
+      (given(cos_sin) && (overlap(pages, *cos_sin) || overlap(pages, *positions))))
+    bad_argument("pages must not overlap the other tensors");
   int* sp = status_ptr(status, device);
   if (T == 0 || heads == 0) return;
   if (row_stride(k) % 8 || row_stride(v) % 8 || ldq % 8 || ldqo % 8) bad_argument("token strides must be multiples of 8 elements");
@@ -260,7 +279,8 @@ void kv_read_int4(at::Tensor pages, at::Tensor slots, at::Tensor k_out, at::Tens
   check_pages(pages, page_size, heads, d, device);
   const int slots64 = check_index(slots, "slots", T, device);
   int* sp = status_ptr(status, device);
-  if (overlap(k_out, v_out) || overlap(k_out, pages) || overlap(v_out, pages)) bad_argument("k_out, v_out and pages must not overlap");
+  if (overlap(k_out, v_out) || overlap(k_out, pages) || overlap(v_out, pages) || overlap(k_out, slots) || overlap(v_out, slots))
+    bad_argument("k_out, v_out, pages and slots must not overlap");
   if (T == 0 || heads == 0) return;
   if (heads > 16384) bad_argument("too many heads");
   const c10::cuda::CUDAGuard guard(k_out.device());
@@ -301,7 +321,7 @@ void kv_attention_int4(at::Tensor q, at::Tensor pages, at::Tensor block_table, a
   const int64_t device = q.get_device();
   check_rows(out, "out", device);
   if (out.sizes() != q.sizes()) bad_argument("out must have the shape of q");
-  if (overlap(out, q)) bad_argument("out must not overlap q");
+  if (rows_overlap(out, q)) bad_argument("out must not overlap q");
   const int64_t T = q.size(0), q_heads = q.size(1), d = q.size(2);
   check_cuda(pages, "pages", at::kByte, device);
   if (pages.dim() != 3) bad_argument("pages must be [num_pages, kv_heads, page_size * (channels + 8)]");
@@ -321,6 +341,8 @@ void kv_attention_int4(at::Tensor q, at::Tensor pages, at::Tensor block_table, a
   } else if (T != B) {
     bad_argument("without q_starts there is one row of q per sequence");
   }
+  if (overlap(out, pages) || overlap(out, block_table) || overlap(out, seq_lens) || (given(q_starts) && overlap(out, *q_starts)))
+    bad_argument("out must not overlap pages, block_table, seq_lens or q_starts");
   int* sp = status_ptr(status, device);
   const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(d));
   if (!(sc > 0) || !(sc <= 1048576.0)) bad_argument("scale must be positive, and at most 2^20");

@@ -412,7 +412,8 @@ int fg_linear_w8a8(const int8_t* x8, const int8_t* W8, const void* x_scales, int
  * of range is left out and FG_ERR_INDEX stored to *status_dev (int in device memory, or NULL: not reported).
  *
  * fg_kv_append_int4: for each of `tokens` rows t with slots[t] >= 0 (negative: a padding row, left out whole), turns
- * k[t] and q[t] by the angles of positions[t], writes q to q_out (fp16, rounded once; q_out may be q) and the rows
+ * k[t] and q[t] by the angles of positions[t], writes q to q_out (fp16, rounded once; q_out may be q, but lie over nothing
+ * else that the call reads or writes; no more may pages) and the rows
  * k[t], v[t] of every head, quantised from the unrounded values, to the cache:
  *     low = fp16(min x), scale = max(fp16((max x - low) / 15), 2^-24), code = clamp(rint((x - low) / scale), 0, 15)
  * A row with an infinity or a NaN in it reads back as NaN.  k, v [tokens, kv_heads, d] and q, q_out
@@ -440,7 +441,7 @@ int fg_kv_read_int4(const void* pages, long long num_pages, int page_size, int k
  * A query that sees nothing (an empty sequence) gives zeros; rows of q outside every sequence leave out as it was; rows of
  * a page number out of range count as absent.  Scores, weights and sums in fp32, weights rounded to fp16 for the product
  * with the codes.  The split over the length depends on the lengths alone: results are reproducible bit by bit.
- * ws: fg_kv_attention_workspace_bytes() of device memory, 256-byte aligned, cleared once with
+ * out must not overlap what the call reads.  ws: fg_kv_attention_workspace_bytes() of device memory, 256-byte aligned, cleared once with
  * fg_kv_attention_workspace_init (a call leaves it ready for the next); one per stream that may run concurrently. */
 size_t fg_kv_attention_workspace_bytes(void);
 int fg_kv_attention_workspace_init(void* ws, size_t ws_bytes, fg_stream_t stream);

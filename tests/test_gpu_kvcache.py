@@ -481,3 +481,73 @@ def test_joins_read_the_partials_of_their_own_call(dev):
         fg.kv_attention_int4(qd, pd, td, ld, out, page)
     torch.cuda.synchronize()
     assert all(torch.equal(out, want[i % 4]) for i, out in enumerate(got))
+
+
+def test_outputs_over_other_operands_are_refused(dev):
+    """What a call writes may not lie over what it reads (nothing is launched); q_out may be q itself."""
+    T, hq, hkv, d, page = 6, 4, 2, 64, 16
+    n = T * hq * d
+    g = torch.Generator().manual_seed(41)
+    half = lambda *s: torch.randn(*s, generator=g).half().to(dev)
+    big = half(4 * n)  # k at 0, v behind it, q at 2 n, room behind
+    k, v, q = big[: T * hkv * d].view(T, hkv, d), big[T * hkv * d: n].view(T, hkv, d), big[2 * n: 3 * n].view(T, hq, d)
+    over = lambda at: big[at: at + n].view(T, hq, d)
+    bytes_ = torch.zeros(1 << 16, dtype=torch.uint8, device=dev)  # pages, and what is put over them
+    pages = bytes_[: 2 * hkv * page * (d + 8)].view(2, hkv, page * (d + 8))
+    in_pages = bytes_[512: 512 + 2 * n].view(torch.half).view(T, hq, d)
+    slots, pos = torch.arange(T, device=dev), torch.arange(T, device=dev)
+    table = rotation_table(8, d)
+    ints = torch.arange(4 * n, device=dev)  # indices, and outputs over them
+    in_ints = ints[:n // 4].view(torch.half).view(T, hq, d)
+    in_table = rotation_table(1024, d)
+    append = lambda q_out, k=k, q=q, slots=slots, cs=table, pos=pos, p=pages: fg.kv_append_int4(k, v, p, slots, page, cs, pos, q, q_out)
+    before = big.clone()
+    for bad in (lambda: append(over(0)), lambda: append(over(T * hkv * d)), lambda: append(over(2 * n - 8)), lambda: append(over(2 * n + 64)),
+                lambda: append(in_pages), lambda: append(in_ints, slots=ints[:T]), lambda: append(in_ints, pos=ints[2:2 + T]),
+                lambda: append(in_table.view(torch.half).flatten()[:n].view(T, hq, d), cs=in_table),
+                lambda: append(None, q=in_pages), lambda: append(None, k=in_pages[:, :hkv].contiguous().copy_(0), q=in_pages),
+                lambda: fg.kv_append_int4(bytes_[:2 * T * hkv * d].view(torch.half).view(T, hkv, d), v, pages, slots, page),
+                lambda: fg.kv_append_int4(k, bytes_[:2 * T * hkv * d].view(torch.half).view(T, hkv, d), pages, slots, page),
+                lambda: fg.kv_append_int4(k, v, pages, bytes_[:8 * T].view(torch.int64), page)):
+        with pytest.raises(ValueError, match="overlap"):
+            bad()
+    assert torch.equal(big, before) and int(pages.max()) == 0
+    block_table, lens, starts = torch.zeros(T, 1, dtype=torch.int32, device=dev), torch.ones(T, dtype=torch.int32, device=dev), torch.arange(T + 1, dtype=torch.int32, device=dev)
+    i32 = torch.zeros(n, dtype=torch.int32, device=dev)
+    in_i32 = i32[: n // 2].view(torch.half).view(T, hq, d)
+    attend = lambda out, q=q, t=block_table, l=lens, s=starts: fg.kv_attention_int4(q, pages, t, l, out, page, s)
+    for bad in (lambda: attend(q), lambda: attend(over(2 * n + 64)), lambda: attend(in_pages), lambda: attend(in_i32, t=i32[:T].view(T, 1)),
+                lambda: attend(in_i32, l=i32[16:16 + T]), lambda: attend(in_i32, s=i32[8:9 + T])):
+        with pytest.raises(ValueError, match="overlap"):
+            bad()
+    room = torch.empty(2 * T * hkv * d, dtype=torch.half, device=dev)
+    with pytest.raises(ValueError, match="overlap"):
+        fg.kv_read_int4(pages, room[: 4 * T].view(torch.int64), room[: T * hkv * d].view(T, hkv, d), room[T * hkv * d:].view(T, hkv, d), page)
+
+
+def test_column_ranges_of_one_buffer_do_not_overlap(dev):
+    """q, k, v, the turned queries and the attention's output side by side in one buffer of rows."""
+    T, hq, hkv, d, page = 5, 4, 1, 64, 16
+    g = torch.Generator().manual_seed(43)
+    wide = torch.randn(T, (3 * hq + 2 * hkv) * d, generator=g).half()
+    ranges = [hq * d, hkv * d, hkv * d, hq * d, hq * d]
+    buf = wide.to(dev)
+    q, k, v, q_out, out = (t.unflatten(1, (-1, d)) for t in buf.split(ranges, 1))
+    cache, table, pos = KVCacheInt4(1, hkv, d, page), rotation_table(16, d), torch.arange(T, device=dev)
+    cache.append(k, v, pos, table, pos, q, q_out)
+    starts = torch.tensor([0, T], dtype=torch.int32, device=dev)
+    block_table, lens = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.tensor([T], dtype=torch.int32, device=dev)
+    cache.attend(q_out, block_table, lens, out, q_starts=starts)
+    want_q = ref.rotate(wide[:, : hq * d].unflatten(1, (-1, d)), table.cpu(), pos.cpu(), False)
+    assert bool(((q_out.cpu().double() - want_q).abs() <= want_q.abs() * ref.HALF_STEP + 2.0 ** -18).all())
+    _check_attention(out, cache.pages.cpu(), [[0]], q_out.cpu(), [T], page, [0, T])
+    assert torch.equal(buf.cpu()[:, : sum(ranges[:3])], wide[:, : sum(ranges[:3])])
+    one = buf[:1]  # a single row
+    q, k, v, q_out, out = (t.unflatten(1, (-1, d)) for t in one.split(ranges, 1))
+    cache.append(k, v, pos[:1], table, pos[:1], q, q_out)
+    cache.attend(q_out, block_table, lens[:1], out)
+    # ranges that share a column do
+    with pytest.raises(ValueError, match="overlap"):
+        cache.append(k, v, pos[:1], table, pos[:1], q, one[:, 8: 8 + hq * d].unflatten(1, (-1, d)))
+    with pytest.raises(ValueError, match="overlap"):
+        cache.attend(buf[:, :hq * d].unflatten(1, (-1, d)), block_table, lens, buf[:, hq * d - 8: 2 * hq * d - 8].unflatten(1, (-1, d)), q_starts=starts)
