@@ -121,9 +121,17 @@ int encode_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const voi
   const cuuint64_t gstride[1] = {(row_stride_elems ? row_stride_elems : inner) * static_cast<uint64_t>(elem_bytes)};
   const cuuint32_t box[2] = {box_inner, box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = enc(tm, dt, 2, const_cast<void*>(base), gdim, gstride, box, estr,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return enc(tm, dt, 2, const_cast<void*>(base), gdim, gstride, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+    // A driver call, unlike the runtime's, does not make the device's context current in a thread that has made no CUDA call yet.
+    int dev = -1;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
   if (r != CUDA_SUCCESS) {
     g_last_cuda = static_cast<int>(r);
     return FG_ERR_CUDA;
