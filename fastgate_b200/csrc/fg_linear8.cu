@@ -4,8 +4,6 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
-#include <array>
-#include <map>
 #include <mutex>
 
 #include "../../include/fastgate_b200.h"
@@ -111,19 +109,20 @@ Tiling choose_tiling(int M, int N, int K, bool gated, int sm_count, int smem_opt
 void cluster_limits(int sm_count, int (&clusters)[3]) {
   for (int i = 0; i < 3; ++i) clusters[i] = (sm_count - sm_count / 8) >> (i + 1);
 }
+constexpr int kMaxDevices = 64;  // as many as fg_capi.cu keeps
 int clusters_at_once(const fg::host::Device& dev, int (&clusters)[3]) {
   static std::mutex mu;
-  static std::map<int, std::array<int, 3>>* known = new std::map<int, std::array<int, 3>>;
+  static int known[kMaxDevices][3];  // (no container: an allocation that fails may not throw out of a C entry point)
+  static bool asked[kMaxDevices];
+  if (dev.index < 0 || dev.index >= kMaxDevices) return FG_ERR_NO_DEVICE;
   std::lock_guard<std::mutex> lk(mu);
-  const auto it = known->find(dev.index);
-  cluster_limits(dev.sm_count, clusters);
-  if (it == known->end()) {
+  int(&found)[3] = known[dev.index];
+  if (!asked[dev.index]) {
     // (Every tiling's ring takes an SM's shared memory, so one kernel speaks for all.)
     const auto kern = fg::fg_gemm8_kernel<1, 64>;
     const int smem = fg::gemm8_smem_bytes(1, 64, stages_of({64, 1, 0.0, 0.0}, dev.smem_optin));
     const int st = fg::host::opt_in_smem(reinterpret_cast<const void*>(kern), smem);
     if (st != FG_OK) return st;
-    std::array<int, 3> found;
     for (int i = 0; i < 3; ++i) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(dev.sm_count / (2 << i) * (2 << i));
@@ -141,11 +140,10 @@ int clusters_at_once(const fg::host::Device& dev, int (&clusters)[3]) {
         return FG_ERR_CUDA;
       }
     }
-    known->emplace(dev.index, found);
-    for (int i = 0; i < 3; ++i) clusters[i] = clusters[i] < found[i] ? clusters[i] : found[i];
-  } else {
-    for (int i = 0; i < 3; ++i) clusters[i] = clusters[i] < it->second[i] ? clusters[i] : it->second[i];
+    asked[dev.index] = true;
   }
+  cluster_limits(dev.sm_count, clusters);
+  for (int i = 0; i < 3; ++i) clusters[i] = clusters[i] < found[i] ? clusters[i] : found[i];
   return FG_OK;
 }
 

@@ -1,5 +1,8 @@
 """linear_int8 against 64 bits: the GEMV and every tiling of the tensor-core kernel, every epilogue, the largest sums, graphs."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -243,3 +246,30 @@ def test_captured_before_any_eager_call(dev):
     want = torch.empty_like(c)
     fg.linear_int8(a[0], a[1], want, a[2], a[3])
     assert torch.equal(c, want) and fg.workspace_status(0) == 0
+
+
+def test_first_calls_from_several_threads():
+    """What a process finds out once about its device is found out by whichever thread comes first."""
+    code = """
+import threading, torch
+import fastgate_b200 as fg
+dev = torch.device("cuda:0")
+g = torch.Generator().manual_seed(1)
+x, w = (torch.randint(-9, 10, (n, 1024), generator=g, dtype=torch.int8).to(dev) for n in (16, 512))
+s = torch.full((16,), 2.0 ** -10, device=dev)
+outs = [torch.empty(16, 512, dtype=torch.half, device=dev) for _ in range(8)]
+torch.cuda.synchronize()
+gate = threading.Barrier(8)
+def run(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        gate.wait()
+        fg.linear_int8(x, w, outs[i], s)
+threads = [threading.Thread(target=run, args=(i,)) for i in range(8)]
+for t in threads: t.start()
+for t in threads: t.join()
+torch.cuda.synchronize()
+want = (x.cpu().double() @ w.cpu().double().T * 2.0 ** -10).half()
+assert all(torch.equal(o.cpu(), want) for o in outs)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)

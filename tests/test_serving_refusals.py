@@ -1,5 +1,7 @@
 """What the serving operators refuse before they touch a device, and the host side of the cache (no GPU needed)."""
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -123,3 +125,11 @@ def test_tilings_of_the_linear_are_launchable():
                         stage = per * (128 + bn) * 128
                         ring = (232448 - 1024 - 64 - 8 * bn) // (stage + 16) * stage
                         assert tiles * splits <= 148 - 148 // 8 and -(-K // 128 // per) >= splits and (splits - 1) * bn * 512 <= ring
+
+
+def test_entry_points_keep_no_containers():
+    """A container's failing allocation would throw through the C interface: the library's own units use none."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fastgate_b200", "csrc")
+    for name in ("fg_norm.cu", "fg_linear8.cu", "fg_kv4.cu", "fg_attn4.cu", "fg_host.h"):
+        with open(os.path.join(csrc, name)) as f:
+            assert not re.search(r"std::(map|unordered_map|vector|string|deque|list|set)\b|\bnew\b [a-z]|\bthrow\b [a-z]+::", re.sub(r"//.*", "", f.read())), name
