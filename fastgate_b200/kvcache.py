@@ -75,8 +75,11 @@ class KVCacheInt4:
         _C.kv_attention_int4(q, self.pages, block_table, seq_lens, out, self.page_size, q_starts, scale, self._status)
 
     def check(self) -> None:
-        """Raises if a call since the last check met an index out of range (waits for the device)."""
+        """Raises if a call since the last check, on whatever stream, met an index out of range (waits for the device)."""
+        wait = torch.cuda.synchronize if self._status.is_cuda else lambda device: None
+        wait(self._status.device)
         status = int(self._status.item())
         if status:
             self._status.zero_()
+            wait(self._status.device)  # calls that follow on other streams report into a cleared word
             raise RuntimeError(f"fastgate_b200: {capi.status_str(status)}")

@@ -551,3 +551,19 @@ def test_column_ranges_of_one_buffer_do_not_overlap(dev):
         cache.append(k, v, pos[:1], table, pos[:1], q, one[:, 8: 8 + hq * d].unflatten(1, (-1, d)))
     with pytest.raises(ValueError, match="overlap"):
         cache.attend(buf[:, :hq * d].unflatten(1, (-1, d)), block_table, lens, buf[:, hq * d - 8: 2 * hq * d - 8].unflatten(1, (-1, d)), q_starts=starts)
+
+
+def test_check_waits_for_every_stream(dev):
+    """A bad index that a call on another stream meets later than the check is asked for."""
+    cache = KVCacheInt4(2, 1, 64, 16)
+    k, slots = torch.zeros(3, 1, 64, dtype=torch.half, device=dev), torch.tensor([0, 32, 1], device=dev)
+    cache.append(k, k, slots.clamp(max=2))
+    cache.check()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        cache.append(k, k, slots)
+    with pytest.raises(RuntimeError, match="out of range"):
+        cache.check()
+    cache.check()
