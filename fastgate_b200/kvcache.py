@@ -49,6 +49,8 @@ class KVCacheInt4:
         position (a padding row) gets slot -1; a row that the table has no page for, the slot behind the last one, which
         append and read leave out and check() reports."""
         rows, width = block_table.shape
+        if rows == 0 or width == 0:  # no page at all
+            return torch.where(positions >= 0, self.pages.shape[0] * self.page_size, -1).long()
         seq, at = sequence.long(), positions.long().clamp(min=0)
         nth = at // self.page_size
         page = block_table[seq.clamp(0, rows - 1), nth.clamp(max=width - 1)].long()

@@ -107,6 +107,15 @@ def test_slots_of_rows_without_a_page():
     assert got.tolist() == [96, 256, 63, 256, 256, 256, -1]
 
 
+@pytest.mark.parametrize("shape", [(0, 3), (3, 0), (0, 0)])
+def test_slots_of_an_empty_table(shape):
+    cache, table = KVCacheInt4(8, 2, 64, page_size=32, device="cpu"), torch.zeros(*shape, dtype=torch.int32)
+    for index in (torch.int32, torch.int64):
+        got = cache.slots(table, torch.tensor([0, 1, 0], dtype=index), torch.tensor([0, -1, 70], dtype=index))
+        assert got.dtype == torch.int64 and got.tolist() == [256, -1, 256]
+        assert cache.slots(table, torch.zeros(0, dtype=index), torch.zeros(0, dtype=index)).tolist() == []
+
+
 def test_tilings_of_the_linear_are_launchable():
     """Every choice: a known tile, a cluster only where its tiles fit the card at once, no CTA without a stage of k, the
     followers' sums within the leader's ring."""
