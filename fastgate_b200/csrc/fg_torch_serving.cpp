@@ -204,7 +204,7 @@ void linear_int8(at::Tensor x8, at::Tensor W8, at::Tensor C, at::Tensor x_scales
 void check_pages(const at::Tensor& pages, int64_t page_size, int64_t kv_heads, int64_t d, int64_t device) {
   check_dense(pages, "pages", at::kByte, device);
   if (d != 64 && d != 128) bad_argument("heads of 64 or 128 channels expected");
-  if (page_size < 16 || page_size % 16 != 0 || page_size > (1 << 20)) bad_argument("page_size must be a multiple of 16");
+  if (page_size < 16 || page_size % 16 != 0 || page_size > (1 << 20)) bad_argument("page_size must be a multiple of 16, at most 2^20");
   if (pages.dim() != 3 || pages.size(0) < 1 || pages.size(1) != kv_heads || pages.size(2) != page_size * (d + 8))
     bad_argument("pages must be [num_pages, kv_heads, page_size * (channels + 8)]");
 }

@@ -36,8 +36,8 @@ class KVCacheInt4:
     def __init__(self, num_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda"):
         if head_dim not in (64, 128):
             raise ValueError("fastgate_b200: head_dim must be 64 or 128")
-        if page_size < 16 or page_size % 16:
-            raise ValueError("fastgate_b200: page_size must be a multiple of 16")
+        if page_size < 16 or page_size % 16 or page_size > 1 << 20:
+            raise ValueError("fastgate_b200: page_size must be a multiple of 16, at most 2^20")
         if num_pages < 1 or kv_heads < 1:
             raise ValueError("fastgate_b200: num_pages and kv_heads must be positive")
         self.page_size, self.kv_heads, self.head_dim = page_size, kv_heads, head_dim

@@ -107,6 +107,11 @@ def test_slots_of_rows_without_a_page():
     assert got.tolist() == [96, 256, 63, 256, 256, 256, -1]
 
 
+def test_pages_that_no_operator_takes_are_refused_at_once():
+    with pytest.raises(ValueError, match="at most"):
+        KVCacheInt4(1, 1, 64, page_size=(1 << 20) + 16, device="cpu")
+
+
 @pytest.mark.parametrize("shape", [(0, 3), (3, 0), (0, 0)])
 def test_slots_of_an_empty_table(shape):
     cache, table = KVCacheInt4(8, 2, 64, page_size=32, device="cpu"), torch.zeros(*shape, dtype=torch.int32)
