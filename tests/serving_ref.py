@@ -124,6 +124,15 @@ def attention_tolerance(out, span, top):
     return HALF_STEP * (span + out.abs()) + 2.0 ** -15 * (top + span) + TINY
 
 
+def attention_error(out, span, top):
+    """A bound without the weights' rounding to fp16 (the kernel multiplies what it leaves over as well, so that 2^-22 of a weight is
+    lost): half a step of the output, and what 32-bit scores move.  A score is at most eight truncated sums of sixteen
+    products away from its own, each 2^-23 of at most 15 sk |scale| log2(e) sum|q|, which is below 100 for normal rows of 128 channels and
+    less for 64: 8 * 100 * 2^-23 in log2, a weight moves by ln 2 of that, below 2^-13.8; the exponential and the sums add some
+    2^-21.  Weights that are off by e move the output by at most e times its distance from the values, below top + span."""
+    return HALF_STEP * out.abs() + 2.0 ** -13.8 * (top + span) + TINY
+
+
 def random_pages(g, count, heads, d, page_size, spread=1.0, offset=0.0):
     """A pool whose rows are quantised normal rows (packed here, in 64 bits)."""
     rows = torch.randn(count, heads, page_size // BLOCK, 2, BLOCK, d, generator=g, dtype=F64) * spread + offset

@@ -567,3 +567,87 @@ def test_check_waits_for_every_stream(dev):
     with pytest.raises(RuntimeError, match="out of range"):
         cache.check()
     cache.check()
+
+
+def test_extreme_rows_as_keys_and_as_values(dev):
+    """Constant rows, zero rows, the largest values, the smallest, rows that are not finite: each row reads back alike whether it was
+    stored as a key or as a value, whatever lies beside it."""
+    d, page = 128, 16
+    k = torch.zeros(8, 1, d, dtype=torch.half)
+    k[1], k[2], k[3] = 3.25, -0.0, 65504.0
+    k[4, 0, ::2], k[4, 0, 1::2] = -65504.0, 65504.0
+    k[5, 0, 3], k[6, 0, 3] = float("inf"), float("nan")
+    k[7] = torch.arange(d) * 2.0 ** -24
+    cache, slots = KVCacheInt4(2, 1, d, page), torch.arange(8, device=dev)
+    cache.append(k.to(dev), k.flip(0).contiguous().to(dev), slots)
+    kb, vb = (t.cpu() for t in cache.read(slots))
+    cache.check()
+    vb = vb.flip(0)
+    finite = [0, 1, 2, 3, 4, 7]
+    assert torch.equal(kb[finite], vb[finite]) and bool(torch.isfinite(vb[finite]).all())
+    assert bool(torch.isnan(kb[5:7]).all()) and bool(torch.isnan(vb[5:7]).all())
+    assert torch.equal(vb[:4].float(), k[:4].float())
+    assert float((vb[4].double() - k[4].double()).abs().max()) <= 65504 * 2.0 ** -10
+    _check_rows(vb[7:], k[7:].double())
+
+
+def _check_attention_error(out, pool, table, q, lens, page, starts):
+    want, span, top = ref.attention(q, pool, table, lens, page, starts)
+    err, tol = (out.cpu().to(torch.float64) - want).abs(), ref.attention_error(want, span, top)
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (8, 1), (16, 1), (24, 2), (40, 1)])
+def test_output_error_is_its_own_rounding(hq, hkv, d, dev):
+    """Every column of the tiles of eight and of sixteen, one token and several, in items of one CTA and of many."""
+    lens = [1, 40, 700, 2500]
+    pool, table, q, starts = _case(lens, None, hq, hkv, d, 32, hq + d)
+    _check_attention_error(_attend(pool, table, q, lens, 32, starts, dev), pool, table, q, lens, 32, starts)
+    lens, news = [300, 5, 1200], [3, 5, 2]
+    pool, table, q, starts = _case(lens, news, hq, hkv, d, 16, hq + d + 1)
+    _check_attention_error(_attend(pool, table, q, lens, 16, starts, dev), pool, table, q, lens, 16, starts)
+
+
+@pytest.mark.parametrize("d,hq", [(64, 8), (64, 16), (128, 8), (64, 13)])
+def test_long_sums_of_shared_heads_keep_their_precision(d, hq, dev):
+    """As for one query head per key/value head, with all columns of a tile in use: averages of thousands of values, whose errors
+    together stay below half a step (what is exact but for the last rounding has 0.4 of it)."""
+    n, page, batch = 8000, 16, 20
+    pool, table, _, _ = _case([n], None, hq, 1, d, page, 73)
+    lens = [n] * batch
+    table, q = table.repeat(batch, 1), torch.randn(batch, hq, d, generator=torch.Generator().manual_seed(74)).half()
+    out = _attend(pool, table, q, lens, page, None, dev).cpu().to(torch.float64)
+    want, _, _ = ref.attention(q, pool, table, lens, page)
+    assert float((out - want).norm()) <= 2.0 ** -11 * float(want.norm())
+
+
+def test_graph_destroyed_while_it_runs(dev):
+    """The workspace of a graph goes to the next capture only when nothing uses it any more."""
+    page, lens = 64, [5000]
+    pool, table, q, _ = _case(lens, None, 8, 2, 128, page, 51)
+    pd, td, qd, ld = pool.to(dev), table.to(dev), q.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev)
+    want = torch.empty_like(qd)
+    fg.kv_attention_int4(qd, pd, td, ld, want, page)
+
+    def capture(outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            graph.capture_begin(capture_error_mode="relaxed")
+            for out in outs:
+                fg.kv_attention_int4(qd, pd, td, ld, out, page)
+            graph.capture_end()
+        return graph
+
+    first, later = (torch.zeros(n, *q.shape, dtype=torch.half, device=dev) for n in (1000, 20))
+    graph = capture(first)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        graph.replay()
+    del graph  # a thousand calls are still to run
+    graphs = [capture(later) for _ in range(4)]
+    for g in graphs:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            g.replay()
+    torch.cuda.synchronize()
+    assert bool((first == want).all()) and bool((later == want).all())
