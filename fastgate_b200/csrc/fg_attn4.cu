@@ -10,7 +10,7 @@
 // unpacking.  Measured on B200 (64 / 8 heads of 128 channels): 64 sequences of up to 8000 rows 93.6 us, 4.2 TB/s.  Of the 500
 // cycles that a scheduler spends on 16 rows the tensor pipe is busy 192 and the integer pipe 220, and the two hardly overlap: more
 // warps do not help (twelve an SM 97 us; ten, three of them on one scheduler, 110).  One sequence of 5000 rows (32 / 8 heads)
-// 10.4 us: lengths, table, rows, partial sums, ticket, join, each a trip to L2 or memory.
+// 10.9 us: lengths, table, rows, partial sums, ticket, join, each a trip to L2 or memory.
 // What this kernel does about the unpacking:
 //   - A code's four bits, masked in place, ARE an fp16 number: bits 0-3 of a half are the subnormal code * 2^-24, bits 4-7
 //     code * 2^-20.  The tensor core multiplies subnormals exactly, so unpacking is one AND per two codes (and one shift
@@ -19,8 +19,10 @@
 //   - Codes are the 16-row operand of mma.sync.m16n8k16 and the queries that share a key/value head its 8 columns, so a
 //     group of up to eight query heads costs what one does.  S^T = K Q^T leaves P^T in the layout from which
 //     movmatrix makes the second product's operand; nothing goes through shared memory but the cache itself.
-//     (tcgen05.mma takes its operands from shared memory: the codes would have to be written back there as fp16, four
-//     times the bytes that came in.)
+//     (tcgen05.mma could take unpacked codes from tensor memory, written there from registers, and pays where many columns share
+//     them; a few query columns do not, and a kernel for prompts was not built.  6000 new tokens of one sequence, 32 / 8 heads of
+//     128 channels, take 4.3 ms here, 69 TFLOP/s: every eight columns load and unpack the rows again, and units that an item's
+//     last row does not see are still gone through.)
 //   - The softmax's running maximum moves only when a weight exceeds it by more than 2^8 (a warp vote per 32 or 64 rows instead
 //     of a reduction); weights then stay below 2^8 and exact sums are unchanged, since every term uses the same m.
 //     The maximum is taken over log2(p_t sv_t), the weight that is rounded to fp16: its relative error is 2^-11 whatever
@@ -28,7 +30,7 @@
 //   - The fp16 weights alone would leave the output's error at 2.7 times that of an exact result rounded to fp16 (codes are never
 //     negative, so errors of weights meet codes at their full size).  What the rounding of a weight leaves over, again in fp16, is
 //     a second operand of the same product: 1.00 to 1.2 times then.  (64 sequences of up to 8000 rows: 95 us against 86
-//     without; the weights' errors on codes about their middle, which costs 88, still give 1.4 to 1.55.)
+//     without; the weights' errors on codes about their middle, which costs 88, still give 1.4 to 1.55; now 93.6.)
 //   - The tensor core cuts off, towards zero, what does not fit below a 32-bit accumulator; over thousands of rows of
 //     codes that are never negative that adds up (3.3 times the rounding of the output).  Every kDriftSlots slots one more product
 //     takes 7.5 times the weights of those slots off all accumulators, halfway, and its exact amount goes to the 32-bit sums:
@@ -731,7 +733,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) fg_kv_attention_
     auto part_of = [&](uint32_t x) { return first + static_cast<size_t>(2 * x + (x == 0 ? q.first_slot : 0)) * partial_floats(D, COLS); };
     // With L2 most of a microsecond away it is the number of dependent passes that counts: a thread asks for 24 partials of its
     // column at once, maxima included, or for 8 of each of two columns where there are more than one per thread (one sequence of
-    // 5000 rows in 20 parts: 10.4 us, with 8 at once 11.2).
+    // 5000 rows in 20 parts, before dependents were signalled after the wait: 10.4 us, with 8 at once 11.2).
     constexpr int kStep = kAttnThreads / TPC;
     auto join = [&](auto columns) {
       constexpr int Y = decltype(columns)::value;

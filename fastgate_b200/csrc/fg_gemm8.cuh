@@ -17,9 +17,10 @@
 //
 // Persistent: CTAs (pairs) take tiles blockIdx.x, + gridDim.x, ... with the token tiles innermost, so that the tiles in
 // flight share weight rows in L2.  Two accumulators alternate: the epilogue of one tile overlaps the MMAs of the next.
-// The first ring-full of weights is asked for before the previous kernel of the stream has finished (the weight depends
-// on no kernel).  Measured on B200: 3001 x 4096 x 11008 99 us (2.7 POP/s: two waves of 74 pairs and one of narrower tiles),
-// 16 x 28672 x 8192 with the SiLU gate 41 us (5.8 TB/s).  Warps 0-3: epilogue (TMEM lane = token row), 4: copies, 5: MMA.
+// The first ring-full of weights is asked for before the previous kernel of the stream has finished (the weight may not be that
+// kernel's output).  Measured on B200: 3001 x 4096 x 11008 98 us (2.8 POP/s, tensor pipe 77 %: two waves of 74 pairs and one of
+// narrower tiles), 16 x 28672 x 8192 with the SiLU gate 41 us (5.7 TB/s).  Far from their floor: 16 to 128 x 4096 x 4096 7.6 to 8.1 us
+// (2.6 to 2.8) and 16 x 512 x 8192 7.5 (0.7), where each CTA issues four MMAs of 128 token rows for every 4 KB of weight, whatever M.  Warps 0-3: epilogue (TMEM lane = token row), 4: copies, 5: MMA.
 // Sums are exact 32-bit integers.
 #pragma once
 #include "fg_umma.cuh"

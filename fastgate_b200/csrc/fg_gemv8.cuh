@@ -3,13 +3,15 @@
 // A call of this size is a stream of the weight and the latencies around it: one warp takes R weight rows, its lanes stride
 // over k in 16-byte pieces, four dp4a per piece and token row, one integer reduction across the warp at the end.  No
 // ring, no partial tiles, no tickets: nothing stands between the last byte and the output.  The first pieces of the weight
-// are asked for before the previous kernel of the stream has finished (the weight depends on no kernel; the activations
+// are asked for before the previous kernel of the stream has finished (it may not be that kernel's output; the activations
 // are read after griddepcontrol.wait, through L1: every warp of an SM reads the same ones).
-// Measured on B200 (us, one / two rows): 1024 x 1024 1.8 / 2.1, 4096 x 4096 4.7 / 5.1, 11008 x 4096 9.4 / 10.0, 8192 x 8192
-// 12.7 / 13.7, 28672 x 8192 36.8 / 38.9 (the weight at the measured copy bandwidth: 35.9).  Four rows take 7 to 52, against
-// 8 to 38 in the tensor-core kernel: L1 cannot deliver the activations that often.
-// Weights above 60 MB: two rows of the weight per warp halve the reads of x (8192 x 8192 14.8 / 16.9 with one, 28672 x 8192
-// 36.8 / 39.1); below, one row per warp spreads the few rows wider (4096 x 4096 4.6 / 5.8 with two).
+// Measured on B200 (us, one / two token rows, weights from memory, call after call): 1024 x 1024 1.6 / 1.8, 4096 x 4096 4.7 / 5.4,
+// 11008 x 4096 8.9 / 10.0, 8192 x 8192 12.1 / 13.4, 28672 x 8192 35.7 / 38.8 (the weight at the measured copy bandwidth: 35.9; a weight
+// of 17 MB that stays in L2: 3.7).  Four token rows took 7 to 52, against 8 to 38 in the tensor-core kernel: L1 cannot deliver the
+// activations that often.
+// Weights above 60 MB: a warp with two weight rows halves the reads of x (8192 x 8192 12.1 / 13.4, with one row 14.4 / 16.9;
+// 28672 x 8192 35.7 / 38.8 and 36.1 / 38.9).  Below, one weight row a warp spreads the few rows wider (4096 x 4096 4.7 / 5.4, with two
+// 5.0 / 5.7; 11008 x 4096 8.9 / 10.0 and 9.7 / 11.8; 4096 x 11008 alone gains with two tokens, 10.5 / 12.0 and 10.7 / 11.7).
 #pragma once
 #include "fg_w8a8.cuh"
 

@@ -439,10 +439,11 @@ int fg_kv_read_int4(const void* pages, long long num_pages, int page_size, int k
  * seq_lens[b] - n + i and sees the rows up to there:
  *     out = sum_t softmax_t(scale * q . k_t) v_t            0 < scale <= 2^20
  * A query that sees nothing (an empty sequence) gives zeros; rows of q outside every sequence leave out as it was; rows of
- * a page number out of range count as absent.  Scores, weights and sums in fp32, weights rounded to fp16 for the product
- * with the codes.  The split over the length depends on the lengths alone: results are reproducible bit by bit.
- * out must not overlap what the call reads.  ws: fg_kv_attention_workspace_bytes() of device memory, 256-byte aligned, cleared once with
- * fg_kv_attention_workspace_init (a call leaves it ready for the next); one per stream that may run concurrently. */
+ * a page number out of range count as absent.  Scores, weights and sums in fp32; for the product with the codes a weight is
+ * a pair of fp16 numbers, its rounding and what that leaves over.  The same call on the same device gives the same bits;
+ * how a sequence is split depends on all lengths and query ranges of the call, so its last bits may change with its batch.
+ * out must not overlap what the call reads.  ws: fg_kv_attention_workspace_bytes() of device memory, 256-byte aligned, cleared
+ * once with fg_kv_attention_workspace_init (a call leaves it ready for the next); one per stream that may run concurrently. */
 size_t fg_kv_attention_workspace_bytes(void);
 int fg_kv_attention_workspace_init(void* ws, size_t ws_bytes, fg_stream_t stream);
 int fg_kv_attention_int4(const void* q, long long ldq, void* out, long long ldo, long long tokens, int q_heads, int kv_heads, int d,

@@ -651,3 +651,11 @@ def test_graph_destroyed_while_it_runs(dev):
             g.replay()
     torch.cuda.synchronize()
     assert bool((first == want).all()) and bool((later == want).all())
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(128, 8, 2), (64, 12, 1)])
+def test_prompt(d, hq, hkv, dev):
+    """A sequence's first chunk, and a later one behind rows that are there already."""
+    for rows, new in ((600, 600), (900, 333)):
+        pool, table, q, starts = _case([rows], [new], hq, hkv, d, 32, rows + d)
+        _check_attention_error(_attend(pool, table, q, [rows], 32, starts, dev), pool, table, q, [rows], 32, starts)
