@@ -412,11 +412,11 @@ int fg_linear_w8a8(const int8_t* x8, const int8_t* W8, const void* x_scales, int
  * of range is left out and FG_ERR_INDEX stored to *status_dev (int in device memory, or NULL: not reported).
  *
  * fg_kv_append_int4: for each of `tokens` rows t with slots[t] >= 0 (negative: a padding row, left out whole), turns
- * k[t] and q[t] by the angles of positions[t], writes q to q_out (fp16, rounded once; q_out may be q, but lie over nothing
- * else that the call reads or writes; no more may pages) and the rows
- * k[t], v[t] of every head, quantised from the unrounded values, to the cache:
+ * k[t] and q[t] by the angles of positions[t], writes q to q_out (fp16, rounded once) and the rows k[t], v[t] of every
+ * head, quantised from the unrounded values, to the cache:
  *     low = fp16(min x), scale = max(fp16((max x - low) / 15), 2^-24), code = clamp(rint((x - low) / scale), 0, 15)
- * A row with an infinity or a NaN in it reads back as NaN.  k, v [tokens, kv_heads, d] and q, q_out
+ * A row with an infinity or a NaN in it, and a key that is turned below fp16's range, reads back as NaN.  q_out may be q;
+ * neither it nor pages may otherwise overlap what the call reads or writes.  k, v [tokens, kv_heads, d] and q, q_out
  * [tokens, q_heads, d] fp16 with token strides ldk, ldv, ldq, ldqo (elements, multiples of 8), heads dense: column ranges
  * of one fused projection serve as they are.  cos_sin [positions_len, d] fp32 holds cos of the d/2 angles of a position,
  * then sin; interleaved = 0 turns channel pairs (i, i + d/2), 1 pairs (2i, 2i + 1).  cos_sin and positions NULL: no

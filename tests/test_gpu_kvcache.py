@@ -659,3 +659,24 @@ def test_prompt(d, hq, hkv, dev):
     for rows, new in ((600, 600), (900, 333)):
         pool, table, q, starts = _case([rows], [new], hq, hkv, d, 32, rows + d)
         _check_attention_error(_attend(pool, table, q, [rows], 32, starts, dev), pool, table, q, [rows], 32, starts)
+
+
+def test_keys_turned_out_of_range(dev):
+    """A pair of the largest values turned by an eighth: above fp16's range the row saturates, below it the row has an infinity and
+    reads back as NaN, as its fp16 low end says; its neighbours do not notice."""
+    d, page = 64, 16
+    cache = KVCacheInt4(1, 1, d, page)
+    table = torch.zeros(2, d, device=dev)
+    table[0, : d // 2] = 1.0
+    table[1] = 0.5 ** 0.5
+    k = torch.randn(4, 1, d, generator=torch.Generator().manual_seed(1)).half()
+    k[1, 0, 0], k[1, 0, d // 2] = 65504.0, 65504.0    # (0, 92636)
+    k[2, 0, 0], k[2, 0, d // 2] = -65504.0, -65504.0  # (0, -92636)
+    slots, pos = torch.arange(4, device=dev), torch.tensor([0, 1, 1, 0], device=dev)
+    cache.append(k.to(dev), k.to(dev), slots, table, pos)
+    kb, vb = cache.read(slots)
+    cache.check()
+    _check_rows(kb[[0, 3]], k[[0, 3]].double())
+    assert float(kb[1, 0, d // 2]) == 65504.0 and bool(torch.isfinite(kb[1]).all())
+    assert bool(torch.isnan(kb[2]).any()) and not bool(torch.isfinite(kb[2]).any())
+    _check_rows(vb, k.double())

@@ -98,3 +98,40 @@ def test_weight_written_two_calls_earlier(writer, dev):
                 read(x, c)
             torch.cuda.synchronize()
             assert all(torch.equal(c, w) for c in got), (name, x.shape[0])
+
+
+@pytest.mark.parametrize("writer", ["norm", "norm_int8", "linear_int8", "append", "attention"])
+def test_captured_weight_written_two_calls_earlier(writer, dev):
+    """The same three calls in a graph, where the early starts are edges between its nodes."""
+    w16, w8, writers = _writers(dev)
+    weight, write = writers[writer]
+    if weight is w8:
+        x = torch.randint(-9, 10, (16, K), generator=torch.Generator().manual_seed(16), dtype=torch.int8).to(dev)
+        scales = torch.full((16,), 2.0 ** -12, device=dev)
+        read = lambda c: fg.linear_int8(x, w8, c, scales)
+    else:
+        x = _rand(16, 16, K).half().to(dev) / 64
+        read = lambda c: fg.edgemm_m8n128k64x4_bt(x, w16, c)
+    between = _between(dev)
+    want, got = (torch.empty(16, N, dtype=torch.half, device=dev) for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # the stream's workspaces, too
+        write()
+        torch.cuda.synchronize()
+        read(want)
+        for call in between.values():
+            call()
+        torch.cuda.synchronize()
+    for name, call in between.items():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            weight.zero_()
+            write()
+            call()
+            read(got)
+        for _ in range(5):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), name
